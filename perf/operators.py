@@ -137,7 +137,7 @@ def prepare(case, seed):
             torch.pow(10000.0, -torch.arange(0, d, 2, dtype=torch.float64, device="cuda") / d)[None, :]
         state.update(q=randn(B, T, case["q_heads"], d, dtype=dtype), k=randn(B, T, case["k_heads"], d, dtype=dtype),
                      freqs=torch.stack([angle.cos(), angle.sin()], -1).reshape(rows, d).float(),
-                     positions=torch.randint(0, rows, (len(sections), B, T), generator=gen, device="cuda", dtype=torch.int32),
+                     positions=torch.randint(0, rows, (B, T, len(sections)), generator=gen, device="cuda", dtype=torch.int32),
                      sections=sections, half=case["half"], order=case["order"],
                      pair_axis=torch.tensor(_pair_axis(sections, case["order"]), device="cuda"))
     elif case["op"] == "dropout":
@@ -215,7 +215,7 @@ def _random_halfwords(count, seed):
 def _run_plain(s):
     if s["op"] == "rope_axes":
         pairs = s["q"].shape[-1] // 2
-        row = s["positions"].long()[s["pair_axis"]].permute(1, 2, 0)               # (B, T, pairs)
+        row = s["positions"].long()[..., s["pair_axis"]]                           # (B, T, pairs)
         cs = s["freqs"].view(-1, pairs, 2)[row, torch.arange(pairs, device=row.device)][:, :, None]
         return [_rotate(x, cs[..., 0], cs[..., 1], s["half"], s["backward"]) for x in (s["q"], s["k"])]
     if s["op"] == "dropout":
@@ -283,7 +283,7 @@ def exact(case, seed):
             v = torch.stack([v[..., :d // 2], v[..., d // 2:]], -1) if s["half"] else v.view(*v.shape[:-1], d // 2, 2)
             v = torch.view_as_complex(v.contiguous())
             for j in range(d // 2):
-                turn = cs[s["positions"][axis[j]].long(), j]
+                turn = cs[s["positions"][..., axis[j]].long(), j]
                 v[..., j] *= (turn.conj() if s["backward"] else turn)[..., None]
             y = torch.view_as_real(v)
             turned.append(torch.cat([y[..., 0], y[..., 1]], -1) if s["half"] else y.flatten(-2))
