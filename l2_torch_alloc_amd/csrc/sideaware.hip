@@ -433,6 +433,7 @@ struct CompiledKernel {
     int vec_size = 0;           // elements per vector
     bool sided = false;         // built with the sided ownership map
     bool gathered = false;      // inputs 1..3 go through the op's own indexing()
+    bool ragged = false;        // takes arrays that end inside a vector (the op defines RAGGED_TAIL)
     unsigned char in_size[4] = {0, 0, 0, 0}, out_size[4] = {0, 0, 0, 0};   // element bytes per slot, 0: unused
     int wg_threads = 256;       // the workgroup size it was compiled for
     bool failed = false;
@@ -574,6 +575,7 @@ static const CompiledKernel* build_kernel(DeviceContext* ctx, int kernel_id, Ker
         k.vec_size = meta[1];
         k.sided = (meta[5] & 1) != 0;
         k.gathered = (meta[5] & 2) != 0;
+        k.ragged = (meta[5] & 4) != 0;
         for (int j = 0; j < 4; j++) {
             k.in_size[j] = (unsigned char)((meta[6] >> (8 * j)) & 0xff);
             k.out_size[j] = (unsigned char)((meta[7] >> (8 * j)) & 0xff);
@@ -970,7 +972,9 @@ void sideaware_elementwise(int kernel_id, size_t num_bytes,
     if (num_bytes == 0 || (out0 == nullptr && in0 == nullptr)) return;
     DeviceContext* ctx = get_context(device);
     if (!ctx) return;
-    if (!check_vector_alignment("elementwise", out0, in0, num_bytes)) return;
+    // an op that defines RAGGED_TAIL takes any whole number of elements; which ops do is known once
+    // they are compiled
+    if (!check_vector_alignment("elementwise", out0, in0, num_bytes % 16 && kernel_id != 0 ? 0 : num_bytes)) return;
 
     const Tuning t = tuning_snapshot();
     const int variant = variant_for(num_bytes, num_bytes, out0, in0, split_lines(out0, out1, out2, out3), t);
@@ -991,6 +995,16 @@ void sideaware_elementwise(int kernel_id, size_t num_bytes,
     if (!k) k = get_kernel(ctx, kernel_id, variant);
     if (!k) return;
 
+    int ragged = (int)(num_bytes % 16);                    // elements behind the last whole vector
+    if (ragged != 0) {
+        if (!k->ragged && !check_vector_alignment("elementwise", out0, in0, num_bytes)) return;
+        const int element = 16 / k->vec_size;
+        if (ragged % element) {
+            set_error("elementwise: num_bytes (%zu) is not a whole number of %d-byte elements", num_bytes, element);
+            return;
+        }
+        ragged /= element;
+    }
     const long long num_vectors = (long long)(num_bytes / 16);
     const long long slots_wanted = slots_wanted_for(ctx, k, entry->default_groups, parallel_groups, forced_per_side, t);
     unsigned int* feedback = nullptr;
@@ -1017,15 +1031,16 @@ void sideaware_elementwise(int kernel_id, size_t num_bytes,
         plan = plan_launch(base, num_vectors, k->tile_vectors, ctx->num_xcds,
                            stripe_for(num_bytes, ctx->num_xcds, t), t.slot_run, slots_wanted);
     }
+    if (ragged && plan.tail_block < 0) plan.tail_block = 0;   // whole tiles, then a part of a vector: any workgroup may have it
 
     // The kernel's arguments, laid out as the device code declares them (natural alignment, in
     // order: the plan's scalars, the workgroup count, the sideband value, i0, o0 and the feedback
     // word, then what is needed late: the owner of the last tile, the other pointers) and
     // handed to the runtime as one block.
-    struct Args32 { int nv, ft, b0, uc, run; unsigned int r; unsigned int blocks; int val; void* first[3]; int tail; int pad; void* rest[7]; };
-    struct Args64 { long long nv, ft, b0, uc, run; unsigned int r; unsigned int blocks; int val; int pad0; void* first[3]; int tail; int pad; void* rest[7]; };
-    static_assert(offsetof(Args32, first) == 32 && offsetof(Args32, tail) == 56 && offsetof(Args32, rest) == 64 && sizeof(Args32) == 120 &&
-                  offsetof(Args64, first) == 56 && offsetof(Args64, tail) == 80 && offsetof(Args64, rest) == 88 && sizeof(Args64) == 144,
+    struct Args32 { int nv, ft, b0, uc, run; unsigned int r; unsigned int blocks; int val; void* first[3]; int tail; int pad; void* rest[7]; int ragged; int pad1; };
+    struct Args64 { long long nv, ft, b0, uc, run; unsigned int r; unsigned int blocks; int val; int pad0; void* first[3]; int tail; int pad; void* rest[7]; int ragged; int pad1; };
+    static_assert(offsetof(Args32, first) == 32 && offsetof(Args32, tail) == 56 && offsetof(Args32, rest) == 64 && offsetof(Args32, ragged) == 120 &&
+                  offsetof(Args64, first) == 56 && offsetof(Args64, tail) == 80 && offsetof(Args64, rest) == 88 && offsetof(Args64, ragged) == 144,
                   "kernel argument layout");
     union { Args32 a32; Args64 a64; } args;
     size_t args_bytes;
@@ -1038,7 +1053,8 @@ void sideaware_elementwise(int kernel_id, size_t num_bytes,
         a.r = plan.r_word; a.blocks = plan.grid; a.val = sideband_value; a.pad0 = 0; a.tail = plan.tail_block; a.pad = 0;
         std::memcpy(a.first, first, sizeof first);
         std::memcpy(a.rest, rest, sizeof rest);
-        args_bytes = sizeof(Args64);
+        a.ragged = ragged; a.pad1 = 0;
+        args_bytes = k->ragged ? sizeof(Args64) : offsetof(Args64, ragged);
     } else {
         Args32& a = args.a32;
         a.nv = (int)num_vectors;
@@ -1046,7 +1062,8 @@ void sideaware_elementwise(int kernel_id, size_t num_bytes,
         a.r = plan.r_word; a.blocks = plan.grid; a.val = sideband_value; a.tail = plan.tail_block; a.pad = 0;
         std::memcpy(a.first, first, sizeof first);
         std::memcpy(a.rest, rest, sizeof rest);
-        args_bytes = sizeof(Args32);
+        a.ragged = ragged; a.pad1 = 0;
+        args_bytes = k->ragged ? sizeof(Args32) : offsetof(Args32, ragged);   // an argument of ops with a ragged tail only
     }
     void* extra[] = {HIP_LAUNCH_PARAM_BUFFER_POINTER, &args, HIP_LAUNCH_PARAM_BUFFER_SIZE, &args_bytes, HIP_LAUNCH_PARAM_END};
 

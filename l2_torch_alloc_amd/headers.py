@@ -169,6 +169,82 @@ _ROPE_HALF_TYPES = {
 }
 
 
+_VECTOR_OP_SIGNATURE = (
+    "#define CUSTOM_VECTOR_OP\n"
+    "__device__ __forceinline__ void vector_op(size_type vec_idx, int vec_size,\n"
+    "                          o0 *out0, o1 *out1, o2 *out2, o3 *out3,\n"
+    "                          const i0 *in0, const i1 *in1, const i2 *in2, const i3 *in3,\n"
+    "                          int* sideband_memory, int sideband_value) {\n")
+# Half-split pairs: fetching a word from the lane that holds the other halves.
+_ROPE_PARTNER_WORD = (
+    "// A lane holds rope_vec elements of one half of a head; the lane rope_partner_lanes away holds\n"
+    "// the same positions of the other half.  The two split the work by position, not by half: the\n"
+    "// lane of the first half rotates the first rope_vec/2 pairs, its partner the rest, so each\n"
+    "// needs only the table entries of its own pairs.  They trade the elements the other needs\n"
+    "// before the rotation and the results the other stores after it: four 32-bit lane exchanges\n"
+    "// per 16-byte vector in all.\n"
+    "// One 32-bit word of the partner lane.  Distances of 1, 2 and 8 lanes are data-parallel\n"
+    "// moves inside a row of 16 lanes, 16 and 32 lanes are gfx950's row and half-wave swaps: all\n"
+    "// run in the vector ALU.  4 lanes goes through the LDS crossbar.  `upper` says whether this\n"
+    "// lane is the one with the higher number of the two.\n"
+    "__device__ __forceinline__ int rope_partner_word(int v, bool upper) {\n"
+    "    if constexpr (rope_partner_lanes == 1) return __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, false);      // quad_perm:[1,0,3,2]\n"
+    "    else if constexpr (rope_partner_lanes == 2) return __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, false); // quad_perm:[2,3,0,1]\n"
+    "    else if constexpr (rope_partner_lanes == 8) return __builtin_amdgcn_update_dpp(0, v, 0x128, 0xf, 0xf, false); // row_ror:8\n"
+    "    else if constexpr (rope_partner_lanes == 16) {\n"
+    "        const auto r = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);\n"
+    "        return (int)(upper ? r[0] : r[1]);\n"
+    "    } else if constexpr (rope_partner_lanes == 32) {\n"
+    "        const auto r = __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false);\n"
+    "        return (int)(upper ? r[0] : r[1]);\n"
+    "    } else return __shfl_xor(v, rope_partner_lanes);\n"
+    "}\n")
+# Half-split pairs: the body of vector_op, with the (cos, sin) of the lane's pairs in an array the
+# caller names (@CS@) and the signs of the sine products (@KEEP@, @SEND@).
+_ROPE_HALF_ROTATE = (
+    "    constexpr int H = rope_vec / 2;                        // pairs per lane\n"
+    "    constexpr int W = H * (int)sizeof(i0) / 4;             // 32-bit words in half a vector\n"
+    "    const bool second = (int)((vec_idx * vec_size) % rope_dim) >= rope_half;\n"
+    "    // The lane of the first half keeps its lower H elements and gives away the upper H; the lane\n"
+    "    // of the second half the other way round.\n"
+    "    int words[2 * W], mine_w[W], offer[W], got[W];\n"
+    "    __builtin_memcpy(words, in0, 8 * W);\n"
+    "    #pragma unroll\n"
+    "    for (int w = 0; w < W; w++) {\n"
+    "        mine_w[w] = second ? words[W + w] : words[w];\n"
+    "        offer[w] = second ? words[w] : words[W + w];\n"
+    "    }\n"
+    "    #pragma unroll\n"
+    "    for (int w = 0; w < W; w++) got[w] = rope_partner_word(offer[w], second);\n"
+    "    i0 mine[H], theirs[H], keep[H], send[H];\n"
+    "    __builtin_memcpy(mine, mine_w, 4 * W);\n"
+    "    __builtin_memcpy(theirs, got, 4 * W);\n"
+    "    // With m this lane's element of a pair and t the partner's, the first-half lane keeps\n"
+    "    // y1 = m*c - t*s and sends y2 = t*c + m*s; the second-half lane keeps y2 = m*c + t*s and\n"
+    "    // sends y1 = t*c - m*s (backward: the signs swap).  One expression serves both: the sign of\n"
+    "    // the s-products is flipped in the first-half lane, which is exact.\n"
+    "    const unsigned flip = second ? 0u : 0x80000000u;\n"
+    "    #pragma unroll\n"
+    "    for (int i = 0; i < H; i++) {\n"
+    "        const float m = (float)mine[i], t = (float)theirs[i];\n"
+    "        const float c = @CS@[2 * i], s = @CS@[2 * i + 1];\n"
+    "        const float ts = __uint_as_float(__float_as_uint(t * s) ^ flip);\n"
+    "        const float ms = __uint_as_float(__float_as_uint(m * s) ^ flip);\n"
+    "        keep[i] = (o0)(m * c @KEEP@ ts);\n"
+    "        send[i] = (o0)(t * c @SEND@ ms);\n"
+    "    }\n"
+    "    __builtin_memcpy(offer, send, 4 * W);\n"
+    "    #pragma unroll\n"
+    "    for (int w = 0; w < W; w++) got[w] = rope_partner_word(offer[w], second);\n"
+    "    __builtin_memcpy(mine_w, keep, 4 * W);\n"
+    "    #pragma unroll\n"
+    "    for (int w = 0; w < W; w++) {\n"
+    "        words[w] = second ? got[w] : mine_w[w];\n"
+    "        words[W + w] = second ? mine_w[w] : got[w];\n"
+    "    }\n"
+    "    __builtin_memcpy(out0, words, 8 * W);\n")
+
+
 def rope_half_header(T: int, n_heads: int, head_dim: int, dtype: str = "bf16", backward: bool = False,
                      heads_first: bool = False, heads_at_launch: bool = False, unrolled: int | None = 1,
                      evict_input: bool = True, positions: bool = False) -> bytes:
@@ -236,28 +312,7 @@ def rope_half_header(T: int, n_heads: int, head_dim: int, dtype: str = "bf16", b
         "__device__ __forceinline__ void elementwise_op(size_t element_idx, int sideband,\n"
         "                               o0 &out0, o1 &out1, o2 &out2, o3 &out3,\n"
         "                               const i0 &in0, const i1 &in1, const i2 &in2, const i3 &in3) {}\n"
-        "// A lane holds rope_vec elements of one half of a head; the lane rope_partner_lanes away holds\n"
-        "// the same positions of the other half.  The two split the work by position, not by half: the\n"
-        "// lane of the first half rotates the first rope_vec/2 pairs, its partner the rest, so each\n"
-        "// needs only the table entries of its own pairs.  They trade the elements the other needs\n"
-        "// before the rotation and the results the other stores after it: four 32-bit lane exchanges\n"
-        "// per 16-byte vector in all.\n"
-        "// One 32-bit word of the partner lane.  Distances of 1, 2 and 8 lanes are data-parallel\n"
-        "// moves inside a row of 16 lanes, 16 and 32 lanes are gfx950's row and half-wave swaps: all\n"
-        "// run in the vector ALU.  4 lanes goes through the LDS crossbar.  `upper` says whether this\n"
-        "// lane is the one with the higher number of the two.\n"
-        "__device__ __forceinline__ int rope_partner_word(int v, bool upper) {\n"
-        "    if constexpr (rope_partner_lanes == 1) return __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, false);      // quad_perm:[1,0,3,2]\n"
-        "    else if constexpr (rope_partner_lanes == 2) return __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, false); // quad_perm:[2,3,0,1]\n"
-        "    else if constexpr (rope_partner_lanes == 8) return __builtin_amdgcn_update_dpp(0, v, 0x128, 0xf, 0xf, false); // row_ror:8\n"
-        "    else if constexpr (rope_partner_lanes == 16) {\n"
-        "        const auto r = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);\n"
-        "        return (int)(upper ? r[0] : r[1]);\n"
-        "    } else if constexpr (rope_partner_lanes == 32) {\n"
-        "        const auto r = __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false);\n"
-        "        return (int)(upper ? r[0] : r[1]);\n"
-        "    } else return __shfl_xor(v, rope_partner_lanes);\n"
-        "}\n"
+        + _ROPE_PARTNER_WORD +
         "#define CUSTOM_IDX_FUNC\n"
         "__device__ __forceinline__ bool indexing(size_type vec_idx, int vec_size,\n"
         "                         size_type &idx_i0, size_type &idx_i1,\n"
@@ -274,53 +329,8 @@ def rope_half_header(T: int, n_heads: int, head_dim: int, dtype: str = "bf16", b
         "    idx_i3 = 0;\n"
         "    return false;\n"
         "}\n"
-        "#define CUSTOM_VECTOR_OP\n"
-        "__device__ __forceinline__ void vector_op(size_type vec_idx, int vec_size,\n"
-        "                          o0 *out0, o1 *out1, o2 *out2, o3 *out3,\n"
-        "                          const i0 *in0, const i1 *in1, const i2 *in2, const i3 *in3,\n"
-        "                          int* sideband_memory, int sideband_value) {\n"
-        "    constexpr int H = rope_vec / 2;                        // pairs per lane\n"
-        "    constexpr int W = H * (int)sizeof(i0) / 4;             // 32-bit words in half a vector\n"
-        "    const bool second = (int)((vec_idx * vec_size) %% rope_dim) >= rope_half;\n"
-        "    // The lane of the first half keeps its lower H elements and gives away the upper H; the lane\n"
-        "    // of the second half the other way round.\n"
-        "    int words[2 * W], mine_w[W], offer[W], got[W];\n"
-        "    __builtin_memcpy(words, in0, 8 * W);\n"
-        "    #pragma unroll\n"
-        "    for (int w = 0; w < W; w++) {\n"
-        "        mine_w[w] = second ? words[W + w] : words[w];\n"
-        "        offer[w] = second ? words[w] : words[W + w];\n"
-        "    }\n"
-        "    #pragma unroll\n"
-        "    for (int w = 0; w < W; w++) got[w] = rope_partner_word(offer[w], second);\n"
-        "    i0 mine[H], theirs[H], keep[H], send[H];\n"
-        "    __builtin_memcpy(mine, mine_w, 4 * W);\n"
-        "    __builtin_memcpy(theirs, got, 4 * W);\n"
-        "    // With m this lane's element of a pair and t the partner's, the first-half lane keeps\n"
-        "    // y1 = m*c - t*s and sends y2 = t*c + m*s; the second-half lane keeps y2 = m*c + t*s and\n"
-        "    // sends y1 = t*c - m*s (backward: the signs swap).  One expression serves both: the sign of\n"
-        "    // the s-products is flipped in the first-half lane, which is exact.\n"
-        "    const unsigned flip = second ? 0u : 0x80000000u;\n"
-        "    #pragma unroll\n"
-        "    for (int i = 0; i < H; i++) {\n"
-        "        const float m = (float)mine[i], t = (float)theirs[i];\n"
-        "        const float c = in1[2 * i], s = in1[2 * i + 1];\n"
-        "        const float ts = __uint_as_float(__float_as_uint(t * s) ^ flip);\n"
-        "        const float ms = __uint_as_float(__float_as_uint(m * s) ^ flip);\n"
-        "        keep[i] = (o0)(m * c %s ts);\n"
-        "        send[i] = (o0)(t * c %s ms);\n"
-        "    }\n"
-        "    __builtin_memcpy(offer, send, 4 * W);\n"
-        "    #pragma unroll\n"
-        "    for (int w = 0; w < W; w++) got[w] = rope_partner_word(offer[w], second);\n"
-        "    __builtin_memcpy(mine_w, keep, 4 * W);\n"
-        "    #pragma unroll\n"
-        "    for (int w = 0; w < W; w++) {\n"
-        "        words[w] = second ? got[w] : mine_w[w];\n"
-        "        words[W + w] = second ? mine_w[w] : got[w];\n"
-        "    }\n"
-        "    __builtin_memcpy(out0, words, 8 * W);\n"
-        "}\n" % (token, keep_sign, send_sign))
+        % token + _VECTOR_OP_SIGNATURE + _ROPE_HALF_ROTATE.replace("@CS@", "in1").replace("@KEEP@", keep_sign).replace("@SEND@", send_sign)
+        + "}\n")
     return "".join(lines).encode()
 
 
@@ -483,3 +493,246 @@ def fill_header() -> bytes:
         "                               const i0 &in0, const i1 &in1, const i2 &in2, const i3 &in3) {\n"
         "    out0 = sideband;\n}\n"
     ).encode()
+
+
+_ROPE_AXES_HEADS_BITS = 10
+ROPE_AXES_MAX_HEADS = (1 << _ROPE_AXES_HEADS_BITS) - 1
+ROPE_AXES_MAX_ROWS = (1 << (32 - _ROPE_AXES_HEADS_BITS)) - 1
+
+
+def rope_axes_sideband(heads: int, rows: int) -> int:
+    """The sideband value of a launch of :func:`rope_axes_header`: the heads per token of the tensor
+    and the rows of the table, in one signed 32-bit word."""
+    if not 1 <= heads <= ROPE_AXES_MAX_HEADS:
+        raise ValueError("multi-axis RoPE takes 1 to %d heads per token, got %d" % (ROPE_AXES_MAX_HEADS, heads))
+    if not 1 <= rows <= ROPE_AXES_MAX_ROWS:
+        raise ValueError("multi-axis RoPE takes a table of 1 to %d rows, got %d" % (ROPE_AXES_MAX_ROWS, rows))
+    word = heads | (rows << _ROPE_AXES_HEADS_BITS)
+    return word - (1 << 32) if word >= 1 << 31 else word
+
+
+def rope_pair_axes(sections, order: str = "blocks") -> list:
+    """The axis of each rotated pair of a head.  ``sections[a]`` pairs belong to axis a: one block of
+    pairs per axis ("blocks"), or dealt to the axes in turn, an axis whose pairs are used up being
+    passed over ("turns")."""
+    sections = [int(n) for n in sections]
+    if not 1 <= len(sections) <= 3 or min(sections) < 1:
+        raise ValueError("sections are 1 to 3 positive numbers of pairs, got %s" % (tuple(sections),))
+    if order == "blocks":
+        return [a for a, n in enumerate(sections) for _ in range(n)]
+    if order != "turns":
+        raise ValueError("order must be 'blocks' or 'turns'")
+    return [a for turn in range(max(sections)) for a, n in enumerate(sections) if turn < n]
+
+
+def rope_axes_header(head_dim: int, sections, dtype: str = "bf16", half: bool = False, order: str = "blocks",
+                     backward: bool = False, unrolled: int | None = 1) -> bytes:
+    """RoPE whose position has several axes (time, height and width of a patch of a video, say),
+    forward or backward, in place or out of place.
+
+    Pair j of a head is rotated by the table's row ``positions[token][a]`` of the axis a the pair
+    belongs to (:func:`rope_pair_axes`): with (c, s) = ``table[row][j]``,
+    ``out = (x1*c - x2*s, x2*c + x1*s)`` in fp32, each product rounded before the add, exactly as in
+    :func:`rope_header` and :func:`rope_half_header`, whose results these are, bit for bit, where all
+    axes of a token agree.  ``half`` selects half-split pairs (element i with element i + head_dim/2)
+    over neighbouring ones.
+
+    in0/out0: the activation, (tokens, heads, head_dim); in1: the fp32 table, (rows, head_dim/2, 2) of
+    (cos, sin), and in2, in3 the same pointer again (see below); the sideband pointer: int32
+    positions, (tokens, axes); the sideband value: :func:`rope_axes_sideband`.  A position outside
+    [0, rows) reads nothing of the table and makes the pairs of its axis NaN.
+
+    A lane rotates vec/2 pairs (4 of them for 16-bit types), whose cos and sin are 2 * vec/2 floats of
+    one row if all of them belong to one axis.  Where every lane's pairs do (sections of whole
+    multiples of vec/2 pairs, in blocks), one row is read, as by the ops with one position.
+    Elsewhere a lane reads its piece of the row of every axis, through in1, in2 and in3, and selects
+    pair by pair: rows are shared by all heads of a token and come out of the L1 cache, where the
+    additional reads cost little.
+    """
+    if dtype not in _ROPE_HALF_TYPES:
+        raise ValueError("dtype must be 'fp32', 'bf16' or 'fp16'")
+    elem, vec = _ROPE_HALF_TYPES[dtype]
+    unit = vec // 2                                      # pairs a lane rotates
+    pair_axis = rope_pair_axes(sections, order)
+    axes = len(list(sections))
+    pairs = head_dim // 2
+    if head_dim % 2 or len(pair_axis) != pairs:
+        raise ValueError("sections must add up to head_dim/2 = %d pairs, got %s" % (pairs, tuple(sections)))
+    if half:
+        lanes = pairs // vec
+        if pairs % vec or lanes < 1 or lanes > 32 or lanes & (lanes - 1):
+            raise ValueError("with half-split pairs head_dim/2 must be a power-of-two multiple (1..32) of %d elements for %s" % (vec, dtype))
+    elif pairs % unit or pairs > 256:
+        raise ValueError("head_dim/2 must be a multiple of %d, at most 256, for %s" % (unit, dtype))
+    one_axis = all(len(set(pair_axis[i:i + unit])) == 1 for i in range(0, pairs, unit))
+    # two bits per pair, 32 pairs to a 64-bit word, found by comparing the pair's number
+    words = [sum(a << (2 * i) for i, a in enumerate(pair_axis[w:w + 32])) for w in range(0, pairs, 32)]
+    code = "".join("pair < %d ? 0x%xull : " % (32 * (i + 1), w) for i, w in enumerate(words[:-1])) + "0x%xull" % words[-1]
+    keep_sign, send_sign = ("-", "+") if backward else ("+", "-")
+
+    name = "sideaware_rope_axes_%s_%s_%s_%s_d%d_%s" % ("bwd" if backward else "fwd", dtype, "half" if half else "pairs", order, head_dim,
+                                                     "_".join(str(int(n)) for n in sections))
+    inputs = 1 if one_axis else axes                     # table rows a lane reads
+    lines = ["#define KERNEL_NAME %s\n" % name,
+             "typedef %s o0;\ntypedef %s i0;\n" % (elem, elem), _UNUSED,
+             "".join("typedef %s i%d;\n" % ("float" if i <= inputs else "unused", i) for i in (1, 2, 3)),
+             "typedef unused o1, o2, o3;\n"]
+    if unrolled is not None:
+        lines.append("#define UNROLLED %d\n" % unrolled)
+    lines.append("constexpr bool reverse_order = false;\n" + _evict([True]))
+    lines.append(
+        "constexpr int rope_dim = %d;           // elements per head\n"
+        "constexpr int rope_half = %d;          // pairs per head\n"
+        "constexpr int rope_axes = %d;\n"
+        "constexpr int rope_vec = %d;           // elements per 16-byte vector\n"
+        "constexpr int rope_unit = rope_vec / 2; // pairs a lane rotates\n"
+        "constexpr bool rope_half_split = %s;\n"
+        % (head_dim, pairs, axes, vec, "true" if half else "false"))
+    if half:
+        lines.append("constexpr int rope_partner_lanes = %d; // lanes between the two halves of a pair\n" % (pairs // vec))
+    lines.append(
+        "__device__ __forceinline__ void elementwise_op(size_t element_idx, int sideband,\n"
+        "                               o0 &out0, o1 &out1, o2 &out2, o3 &out3,\n"
+        "                               const i0 &in0, const i1 &in1, const i2 &in2, const i3 &in3) {}\n"
+        "// the axes of the pairs from `pair` on, two bits each (a lane's pairs never straddle a word)\n"
+        "__device__ __forceinline__ unsigned int rope_axis_code(int pair) {\n"
+        "    return (unsigned int)((%s) >> (2 * (pair %% 32)));\n"
+        "}\n"
+        "// the first pair this lane rotates, and the positions of its token\n"
+        "__device__ __forceinline__ int rope_first_pair(size_type elem) {\n"
+        "    const int in_head = (int)(elem %% rope_dim);\n"
+        "    if constexpr (rope_half_split) return in_head >= rope_half ? in_head - rope_half + rope_unit : in_head;\n"
+        "    else return in_head / 2;\n"
+        "}\n"
+        "__device__ __forceinline__ const int *rope_positions(size_type elem, const int *mem, int val) {\n"
+        "    const size_type token = elem / rope_dim / (size_type)((unsigned int)val & %du);\n"
+        "    return mem + token * rope_axes;\n"
+        "}\n"
+        "__device__ __forceinline__ bool rope_in_table(int position, int val) {\n"
+        "    return (unsigned int)position < ((unsigned int)val >> %d);\n"
+        "}\n"
+        % (code, ROPE_AXES_MAX_HEADS, _ROPE_AXES_HEADS_BITS))
+    # indices count groups of rope_vec floats: the (cos, sin) of rope_unit pairs
+    if one_axis:
+        lookup = ("    const int position = token[rope_axis_code(pair) & 3u];\n"
+                  "    idx_i1 = ((size_type)(rope_in_table(position, val) ? position : 0) * rope_half + pair) / rope_unit;\n"
+                  "    idx_i2 = 0;\n"
+                  "    idx_i3 = 0;\n")
+    else:
+        lookup = "".join(
+            "    idx_i%d = ((size_type)(rope_in_table(token[%d], val) ? token[%d] : 0) * rope_half + pair) / rope_unit;\n" % (a + 1, a, a)
+            for a in range(axes)) + "    idx_i3 = 0;\n" * (axes == 2)
+    lines.append(
+        "#define CUSTOM_IDX_FUNC\n"
+        "__device__ __forceinline__ bool indexing(size_type vec_idx, int vec_size,\n"
+        "                         size_type &idx_i0, size_type &idx_i1,\n"
+        "                         size_type &idx_i2, size_type &idx_i3, int* mem, int val) {\n"
+        "    const size_type elem = vec_idx * vec_size;\n"
+        "    const int pair = rope_first_pair(elem);\n"
+        "    const int *token = rope_positions(elem, mem, val);\n"
+        "    idx_i0 = vec_idx;\n" + lookup +
+        "    return false;\n"
+        "}\n")
+    angles = (
+        "    // the (cos, sin) of this lane's pairs\n"
+        "    const int pair = rope_first_pair(vec_idx * vec_size);\n"
+        "    const int *token = rope_positions(vec_idx * vec_size, sideband_memory, sideband_value);\n"
+        "    const unsigned int axis = rope_axis_code(pair);\n"
+        "    const float outside = __builtin_nanf(\"\");\n"
+        "    float cs[rope_vec];\n")
+    if one_axis:
+        angles += (
+            "    const bool ok = rope_in_table(token[axis & 3u], sideband_value);\n"
+            "    #pragma unroll\n"
+            "    for (int i = 0; i < rope_vec; i++) cs[i] = ok ? in1[i] : outside;\n")
+    else:
+        angles += "".join("    const bool ok%d = rope_in_table(token[%d], sideband_value);\n" % (a, a) for a in range(axes))
+        pick = "ok0 ? in1[i] : outside"
+        for a in range(1, axes):
+            pick = "a == %du ? (ok%d ? in%d[i] : outside) : (%s)" % (a, a, a + 1, pick)
+        angles += (
+            "    #pragma unroll\n"
+            "    for (int i = 0; i < rope_vec; i++) {\n"
+            "        const unsigned int a = (axis >> (i / 2 * 2)) & 3u;\n"
+            "        cs[i] = %s;\n"
+            "    }\n" % pick)
+    if half:
+        body = _ROPE_HALF_ROTATE.replace("@CS@", "cs").replace("@KEEP@", keep_sign).replace("@SEND@", send_sign)
+        lines.append(_ROPE_PARTNER_WORD)
+    else:
+        body = (
+            "    #pragma unroll\n"
+            "    for (int i = 0; i < rope_unit; i++) {\n"
+            "        const float re = (float)in0[2 * i], im = (float)in0[2 * i + 1];\n"
+            "        const float c = cs[2 * i], s = cs[2 * i + 1];\n"
+            "        out0[2 * i] = (o0)(re * c %s im * s);\n"
+            "        out0[2 * i + 1] = (o0)(im * c %s re * s);\n"
+            "    }\n" % (send_sign, keep_sign))
+    lines.append(_VECTOR_OP_SIGNATURE + angles + body + "}\n")
+    return "".join(lines).encode()
+
+
+def dropout_header(dtype: str = "bf16", residual: bool = False, unrolled: int | None = 1) -> bytes:
+    """Dropout whose mask is computed, not stored: ``y = [residual +] (keep ? x * scale : 0)``, in fp32,
+    each operation rounded, once more on the way to 16-bit storage.  The backward pass is the same op
+    on the gradient, without the residual.
+
+    Element e takes 16 random bits: half word e % 8 (low half of a word first) of the four words that
+    Philox4x32 with 7 rounds makes of the counter (e / 8, offset) under the key `seed`, 64 bits each.
+    (Philox: Salmon, Moraes, Dror and Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011; seven
+    is the number of rounds from which the paper reports that the generator passes all tests of
+    BigCrush.)  The element is kept when they are not below the threshold, the probability to drop in units
+    of 2^-16: the sideband value, 0 ... 65536.  scale = 65536 / (65536 - threshold), the reciprocal of
+    the share that the rounded threshold really keeps.  Dropped elements contribute exactly 0, also
+    where x is infinite or NaN.
+
+    in0/out0: the activation; in1: the residual, if any; the sideband pointer: seed and offset, two
+    64-bit words.  The mask depends on seed, offset, threshold and the element's index alone, not on
+    its type, so the gradient may be of another type than the activation was.
+
+    One run of the generator serves the 8 elements of a 16-byte vector of 16-bit type.  It is what this op
+    computes: 14 products of 32 by 32 bits, against 32 bytes moved; ten rounds would make it the bound.
+    """
+    if dtype not in _ROPE_HALF_TYPES:
+        raise ValueError("dtype must be 'fp32', 'bf16' or 'fp16'")
+    elem, vec = _ROPE_HALF_TYPES[dtype]
+    lines = ["#define KERNEL_NAME sideaware_dropout%s_%s\n" % ("_residual" if residual else "", dtype),
+             "#define RAGGED_TAIL\n"
+             "typedef %s o0;\ntypedef %s i0;\n" % (elem, elem), _UNUSED,
+             "typedef %s i1;\ntypedef unused o1, o2, o3, i2, i3;\n" % (elem if residual else "unused")]
+    if unrolled is not None:
+        lines.append("#define UNROLLED %d\n" % unrolled)
+    lines.append("constexpr bool reverse_order = false;\n" + _evict([True, residual]))
+    first = "r[e / 2]" if vec == 8 else "(odd ? r[2 + e / 2] : r[e / 2])"
+    lines.append(
+        "__device__ __forceinline__ void elementwise_op(size_t element_idx, int sideband,\n"
+        "                               o0 &out0, o1 &out1, o2 &out2, o3 &out3,\n"
+        "                               const i0 &in0, const i1 &in1, const i2 &in2, const i3 &in3) {}\n"
+        + _VECTOR_OP_SIGNATURE +
+        "    const unsigned int threshold = (unsigned int)sideband_value;\n"
+        "    const float scale = threshold < 65536u ? 65536.0f / (float)(65536u - threshold) : 0.0f;\n"
+        "    const unsigned int *state = (const unsigned int*)sideband_memory;\n"
+        "    unsigned int k0 = state[0], k1 = state[1];\n"
+        "    const unsigned long long block = (unsigned long long)vec_idx * %d / 8;      // vec_size elements a vector, 8 a block\n"
+        "    unsigned int r[4] = {(unsigned int)block, (unsigned int)(block >> 32), state[2], state[3]};\n"
+        "    #pragma unroll\n"
+        "    for (int i = 0; i < 7; i++) {\n"
+        "        const unsigned long long a = (unsigned long long)r[0] * 0xD2511F53u, b = (unsigned long long)r[2] * 0xCD9E8D57u;\n"
+        "        r[0] = (unsigned int)(b >> 32) ^ r[1] ^ k0;\n"
+        "        r[1] = (unsigned int)b;\n"
+        "        r[2] = (unsigned int)(a >> 32) ^ r[3] ^ k1;\n"
+        "        r[3] = (unsigned int)a;\n"
+        "        k0 += 0x9E3779B9u;\n"
+        "        k1 += 0xBB67AE85u;\n"
+        "    }\n"
+        "    const bool odd = (vec_idx & 1) != 0;                 // of two 4-element vectors, the second half of a block\n"
+        "    (void)odd;\n"
+        "    #pragma unroll\n"
+        "    for (int e = 0; e < %d; e++) {\n"
+        "        const unsigned int word = %s;\n"
+        "        const unsigned int bits = (e & 1) ? word >> 16 : word & 0xffffu;\n"
+        "        const float kept = bits >= threshold ? (float)in0[e] * scale : 0.0f;\n"
+        "        out0[e] = (o0)(%skept);\n"
+        "    }\n"
+        "}\n" % (vec, vec, first, "(float)in1[e] + " if residual else ""))
+    return "".join(lines).encode()

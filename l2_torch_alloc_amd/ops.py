@@ -27,6 +27,8 @@ _HEADER_BUILDERS = {
     "mxfp8_quantize": headers.mxfp8_quantize_header,
     "mxfp8_dequantize": headers.mxfp8_dequantize_header,
     "fill": headers.fill_header,
+    "rope_axes": headers.rope_axes_header,
+    "dropout": headers.dropout_header,
 }
 
 
@@ -156,6 +158,7 @@ def elementwise_batch(kernel_id: int, segments) -> None:
     ``(num_bytes, outs, ins, sideband_tensor_or_None, sideband_value)`` with ``outs`` / ``ins``
     sequences of up to four tensors (or None)."""
     arr = (_Segment * len(segments))()
+    first = next((t for seg in segments for t in list(seg[1]) + list(seg[2]) if t is not None), None)
     for seg, (num_bytes, outs, ins, sideband, value) in zip(arr, segments):
         seg.num_bytes = num_bytes
         for i, t in enumerate(outs):
@@ -164,7 +167,7 @@ def elementwise_batch(kernel_id: int, segments) -> None:
             seg.inp[i] = wrapper._check(t, "in%d" % i) or None
         seg.sideband_memory = sideband.data_ptr() if sideband is not None else None
         seg.sideband_value = int(value)
-    device, stream = wrapper._device_and_stream()
+    device, stream = wrapper._device_and_stream(first)      # where the arrays live, the current device or not
     wrapper.library().sideaware_elementwise_batch(kernel_id, len(arr), arr, device, stream)
 
 
@@ -271,6 +274,122 @@ def rope_half_forward_many(tensors, freqs, backward: bool = False, positions=Non
     kid = _kernel("rope_half", (T, 0, head_dim, dtype, backward), (("heads_at_launch", True),))
     elementwise_batch(kid, [(t.numel() * t.element_size(), [t], [t, freqs], None, t.shape[2]) for t in tensors])
     return tensors
+
+
+def freqs_cis_axes_table(sections, end: int, theta: float, order: str = "blocks") -> torch.Tensor:
+    """(end, head_dim) fp32 table on the host, as :func:`freqs_cis_table` lays it out, for axes that
+    each have a geometric series of frequencies of their own: the i-th pair of axis a turns by
+    ``t * theta^(-i/sections[a])``.  (:func:`freqs_cis_table` itself is the table for axes that share one
+    series over all pairs.)  Angles in 64 bits, rounded once."""
+    axis = headers.rope_pair_axes(sections, order)
+    seen = [0] * len(sections)
+    freq = []
+    for a in axis:
+        freq.append(float(theta) ** (-seen[a] / sections[a]))
+        seen[a] += 1
+    angle = torch.arange(end, dtype=torch.float64)[:, None] * torch.tensor(freq, dtype=torch.float64)[None, :]
+    return torch.stack([angle.cos(), angle.sin()], -1).reshape(end, 2 * len(axis)).float()
+
+
+def _rope_axes_many(tensors, freqs, positions, sections, half: bool, order: str, backward: bool, outs):
+    tensors = list(tensors)
+    outs = tensors if outs is None else list(outs)
+    first = tensors[0]
+    assert first.dim() == 4, "activations are (B, T, heads, head_dim)"
+    B, T, _, head_dim = first.shape
+    dtype = _ROPE_DTYPES.get(first.dtype)
+    if dtype is None:
+        raise TypeError("RoPE storage is float32, bfloat16 or float16")
+    sections = tuple(int(n) for n in sections)
+    assert freqs.dtype == torch.float32 and freqs.dim() == 2 and freqs.shape[1] == head_dim, \
+        "the table is float32, (rows, head_dim)"
+    assert positions.dtype == torch.int32 and positions.is_contiguous(), "positions are a contiguous int32 tensor"
+    assert tuple(positions.shape) in ((B, T, len(sections)), (B * T, len(sections))), \
+        "positions are (B, T, axes): one row of the table for each axis of every token"
+    assert len(outs) == len(tensors), "one output per tensor"
+    for t, o in zip(tensors, outs):
+        assert t.dim() == 4 and t.shape[:2] == first.shape[:2] and t.shape[3] == head_dim and t.dtype == first.dtype, \
+            "tensors share B, T, head_dim and dtype"
+        assert o.shape == t.shape and o.dtype == t.dtype, "an output is like its tensor"
+        assert t.device == o.device == first.device, "tensors and outputs live on one device"
+    assert positions.device == first.device and freqs.device == first.device, "table and positions live on the activations' device"
+    kid = _kernel("rope_axes", (head_dim, sections, dtype, bool(half), order, backward))
+    work = [(t, o) for t, o in zip(tensors, outs) if t.numel()]
+    if work:
+        elementwise_batch(kid, [(t.numel() * t.element_size(), [o], [t, freqs, freqs, freqs], positions,
+                                 headers.rope_axes_sideband(t.shape[2], freqs.shape[0])) for t, o in work])
+    return outs
+
+
+def rope_axes_forward_many(tensors, freqs, positions, sections, half: bool = False, order: str = "blocks", outs=None):
+    """RoPE with a position of 1 to 3 axes (the time, height and width of an image's or video's patch) of
+    several (B, T, heads, head_dim) tensors in ONE launch: q and k of a grouped-query model (different
+    head counts, same B, T, head_dim and dtype).  In place unless ``outs`` is given; returns the outputs.
+
+    ``freqs``: the (rows, head_dim) fp32 table of the ops with one position (``freqs_cis_table``, or
+    ``freqs_cis_axes_table`` for axes with frequencies of their own), with a row for every position that
+    occurs.  ``positions``: int32 (B, T, axes), contiguous; a position outside the table makes the pairs of
+    its axis NaN.  ``sections``: how many of a head's head_dim/2 pairs each axis turns: in blocks of
+    consecutive pairs (``order="blocks"``) or dealt to the axes in turn (``"turns"``).  ``half``: half-split
+    pairs (element i with element i + head_dim/2), as :func:`rope_half_forward` has them, instead of
+    neighbouring ones."""
+    return _rope_axes_many(tensors, freqs, positions, sections, half, order, False, outs)
+
+
+def rope_axes_backward_many(tensors, freqs, positions, sections, half: bool = False, order: str = "blocks", outs=None):
+    """The gradients of :func:`rope_axes_forward_many` (``tensors`` are those of its outputs): the rotation
+    by the opposite angles."""
+    return _rope_axes_many(tensors, freqs, positions, sections, half, order, True, outs)
+
+
+def rope_axes_forward(x, freqs, positions, sections, out=None, half: bool = False, order: str = "blocks"):
+    """:func:`rope_axes_forward_many` of one tensor.  In place unless ``out`` is given."""
+    return _rope_axes_many([x], freqs, positions, sections, half, order, False, None if out is None else [out])[0]
+
+
+def rope_axes_backward(dout, freqs, positions, sections, out=None, half: bool = False, order: str = "blocks"):
+    return _rope_axes_many([dout], freqs, positions, sections, half, order, True, None if out is None else [out])[0]
+
+
+def dropout_threshold(p: float) -> int:
+    """The probability to drop in units of 2^-16, rounded to nearest: what the dropout ops work with."""
+    if not 0.0 <= p <= 1.0:
+        raise ValueError("the probability to drop lies in [0, 1], got %r" % (p,))
+    return int(math.floor(p * 65536.0 + 0.5))
+
+
+def _dropout(x: torch.Tensor, p: float, seed: torch.Tensor, residual: Optional[torch.Tensor], out: Optional[torch.Tensor]):
+    threshold = dropout_threshold(p)
+    dtype = _ROPE_DTYPES.get(x.dtype)
+    if dtype is None:
+        raise TypeError("dropout storage is float32, bfloat16 or float16")
+    assert seed.dtype == torch.int64 and seed.numel() == 2 and seed.is_contiguous() and seed.device == x.device, \
+        "the seed is an int64 tensor of two values (seed, offset) on the activations' device"
+    if residual is not None:
+        assert residual.shape == x.shape and residual.dtype == x.dtype and residual.device == x.device, \
+            "the residual is like the activation"
+    if out is None:
+        out = torch.empty_like(x)
+    assert out.shape == x.shape and out.dtype == x.dtype and out.device == x.device, "the output is like the activation"
+    if x.numel():
+        kid = _kernel("dropout", (dtype, residual is not None))
+        _elementwise(kid, out, None, None, None, x, residual, None, None, seed, threshold, 0, 0)
+    return out
+
+
+def dropout_forward(x, p: float, seed, residual=None, out=None):
+    """``x / (1 - p)`` where an element is kept and 0 where it is dropped (with probability ``p``, rounded to
+    a multiple of 2^-16), plus ``residual`` if one is given, rounded once to the tensors' type.  The mask
+    is computed from the element's index and ``seed``, an int64 device tensor (seed, offset), and never
+    stored: pass the same two to :func:`dropout_backward`.  A launch captured into a graph reads the
+    tensor at every replay, so advancing the offset in place gives each replay a new mask.
+    ``x`` may have any number of elements.  ``out`` may be ``x`` or ``residual``."""
+    return _dropout(x, p, seed, residual, out)
+
+
+def dropout_backward(dout, p: float, seed, out=None):
+    """The gradient of :func:`dropout_forward` with respect to ``x`` (that of the residual is ``dout``)."""
+    return _dropout(dout, p, seed, None, out)
 
 
 def scale_bias_bf16(x: torch.Tensor, scale_bias: torch.Tensor, out: Optional[torch.Tensor] = None):
