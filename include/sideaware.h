@@ -59,7 +59,8 @@ int sideaware_create_kernel(const char* header);
 int sideaware_create_kernel_advanced(const char* header, bool precompile, int default_num_groups);
 
 /* sideaware.cu:1358.  num_bytes is the length of the array whose elements are the wider of
- * (i0, o0); it and the in0/out0 pointers must be multiples of 16.  parallel_groups > 0 fixes
+ * (i0, o0); it and the in0/out0 pointers must be multiples of 16 (an op whose header defines RAGGED_TAIL,
+ * an addition, takes any whole number of elements).  parallel_groups > 0 fixes
  * the workgroups per CU, forced_per_side > 0 the CUs used per XCD.  Returns at once when
  * num_bytes is 0 or both in0 and out0 are null. */
 void sideaware_elementwise(int kernel_id, size_t num_bytes,
@@ -125,6 +126,31 @@ typedef struct sideaware_segment {
  * num_bytes 0 are skipped; more than 8 segments go out as several launches. */
 void sideaware_elementwise_batch(int kernel_id, int num_segments, const sideaware_segment* segments,
                                  int device, sideaware_stream_t stream);
+
+/* Group norm with an activation over an array (batch, pixels, channels), channels last (an addition):
+ *   mean and var over the pixels and the channels of one group of one sample, r = 1/sqrt(var + eps),
+ *   out = act((x - mean) * r * weight + bias).
+ * dtype of x, out, dout and dx: 0 fp32, 1 bf16, 2 fp16.  weight, bias and their gradients, `channels` long
+ * each, are fp32 if weight_fp32 is not 0 and of the arrays' type otherwise; a null weight is 1, a null
+ * bias 0.  activation: 0 none, 1 SiLU (z / (1 + e^-z)).  stats is (batch, groups, 2) fp32, (mean, r):
+ * written by the forward call, read by the backward one.  All sums are kept in 32 bits or more, in an
+ * order that does not depend on the run: the same call gives the same bits.
+ * out may be x, and dx may be dout (or x).  dweight and dbias may be null.
+ * The workspace holds partial sums between a call's launches: at least sideaware_group_norm_workspace()
+ * bytes (0 where the call needs none, and on an error), with nothing to be cleared; calls that may overlap
+ * (on different streams, or captured into different graphs) each need their own.
+ * Arrays and workspace start on multiples of 16 bytes.  Returns 0, -1 for a bad argument, or a HIP error
+ * code; the message is in sideaware_last_error. */
+size_t sideaware_group_norm_workspace(long long batch, long long pixels, int channels, int groups, int dtype, int backward, int device);
+int sideaware_group_norm_forward(void* out, float* stats, const void* x, const void* weight, const void* bias,
+                                 long long batch, long long pixels, int channels, int groups, float eps, int activation,
+                                 int dtype, int weight_fp32, void* workspace, size_t workspace_bytes,
+                                 int device, sideaware_stream_t stream);
+int sideaware_group_norm_backward(void* dx, void* dweight, void* dbias, const void* dout, const void* x,
+                                  const void* weight, const void* bias, const float* stats,
+                                  long long batch, long long pixels, int channels, int groups, int activation,
+                                  int dtype, int weight_fp32, void* workspace, size_t workspace_bytes,
+                                  int device, sideaware_stream_t stream);
 
 /* Upper bound on the device bytes the pool may hold (0 = none): a request that would pass it is
  * answered like one the device refused (caches are given back, then null). */

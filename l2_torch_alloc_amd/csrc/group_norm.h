@@ -1,0 +1,147 @@
+// Group norm with an activation over (batch, pixels, channels) arrays whose channels lie last: how the work
+// is cut (plain C++, shared with the CPU tests) and the launch functions (group_norm.hip).
+//
+// Vocabulary:
+//   vector   `vec` channels of one pixel, 16 bytes at most: the widest power of two that divides the row
+//   slab     consecutive whole groups of channels, a whole number of vectors: one workgroup's share of a row
+//   slice    the part of a slab a workgroup walks at a time, one vector per lane (nearly always all of it)
+//   chunk    consecutive pixels of one sample: one workgroup's share of the pixels
+//   rows     pixels a workgroup works on side by side
+#pragma once
+
+#include <cstddef>
+#include <cstdint>
+
+namespace sideaware {
+
+enum GroupNormType { kGroupNormFp32 = 0, kGroupNormBf16 = 1, kGroupNormFp16 = 2 };
+enum GroupNormActivation { kGroupNormNone = 0, kGroupNormSilu = 1 };
+
+struct GroupNormPlan {
+    int vec = 1;                    // channels per vector
+    int row_vectors = 0;            // vectors per pixel
+    int group_channels = 0;
+    int slab_vectors = 0, slabs = 0;
+    int slab_groups = 0;            // groups of a (full) slab
+    int slice_vectors = 0;          // vectors of a slice: lanes side by side
+    int rows = 1;
+    int threads = 64;
+    long long chunk_pixels = 0;
+    int chunks = 1;                 // per sample; 1: sums and application in one launch
+    long long batch_blocks = 1;     // one launch: workgroups share out the samples of a slab, sample n to n % batch_blocks
+    size_t lds_bytes = 0;
+    // workspace: doubles of the groups' sums [sample][slab][chunk][group of slab][2], then, backward,
+    // floats of the channels' sums [row][2][channel], a row for each (sample or batch block, chunk)
+    size_t group_part_bytes = 0;
+    long long channel_rows = 0;
+    size_t workspace_bytes = 0;
+    long long blocks = 0;           // workgroups of a launch over the array
+    int param_blocks = 0;           // workgroups that add up the channels' sums
+    bool ok = false;
+};
+
+constexpr int kGroupNormMaxThreads = 1024;
+constexpr int kGroupNormMaxSlice = 512;           // vectors: with 8 channels of doubles each, 32 KiB of LDS
+constexpr int kGroupNormMaxSlabGroups = 256;
+constexpr int kGroupNormParamChannels = 64;       // channels per workgroup that adds up their sums
+constexpr long long kGroupNormMaxLanePixels = 256;
+
+inline long long gn_ceil(long long a, long long b) { return (a + b - 1) / b; }
+
+inline GroupNormPlan plan_group_norm(long long batch, long long pixels, int channels, int groups, int element_bytes, bool backward,
+                                     int num_cus) {
+    GroupNormPlan p;
+    if (batch < 1 || pixels < 1 || channels < 1 || groups < 1 || channels % groups || num_cus < 1) return p;
+    p.vec = 16 / element_bytes;
+    while (channels % p.vec) p.vec /= 2;
+    p.row_vectors = channels / p.vec;
+    p.group_channels = channels / groups;
+    // the smallest slab: whole groups and whole vectors (both divide the row, so it does too)
+    int unit = p.group_channels;
+    while (unit % p.vec) unit += p.group_channels;
+    const int unit_vectors = unit / p.vec, unit_groups = unit / p.group_channels, units = channels / unit;
+
+    auto cut = [&](int m) {                        // slabs of m units
+        p.slab_vectors = m * unit_vectors;
+        p.slab_groups = m * unit_groups;
+        p.slabs = (int)gn_ceil(units, m);
+        p.slice_vectors = p.slab_vectors < kGroupNormMaxSlice ? p.slab_vectors : kGroupNormMaxSlice;
+        const long long most_rows = kGroupNormMaxThreads / p.slice_vectors;
+        p.rows = (int)(pixels < most_rows ? pixels : most_rows);
+    };
+    const int most_units = unit_groups * units <= kGroupNormMaxSlabGroups ? units : kGroupNormMaxSlabGroups / unit_groups;
+
+    // One launch where a sample's part of the smallest slab is little: a workgroup then reads it a second
+    // time out of its caches.  Else the pixels are cut into chunks as well, and a second launch applies
+    // what the first one summed.
+    const long long unit_bytes = pixels * unit_vectors * p.vec * element_bytes;
+    if (unit_bytes <= (128 << 10)) {
+        int m = 1;
+        // wider slabs while there are workgroups enough without, up to 512 bytes of a row
+        while (2 * m <= most_units && 2 * m * unit_vectors <= 32 && batch * gn_ceil(units, 2 * m) >= 2 * num_cus &&
+               2 * m * unit_bytes <= (128 << 10))
+            m *= 2;
+        cut(m);
+        p.chunks = 1;
+        p.chunk_pixels = pixels;
+        const long long want = gn_ceil(4ll * num_cus, p.slabs);
+        p.batch_blocks = batch < want ? batch : want;
+    } else {
+        int m = most_units;
+        while (true) {
+            cut(m);
+            const long long step = p.rows;
+            const long long want = gn_ceil(2ll * num_cus, batch * p.slabs);
+            long long most = gn_ceil(pixels, 4 * step);            // at least four pixels a lane
+            if (most < 1) most = 1;
+            long long k = want < most ? want : most;
+            const long long least = gn_ceil(pixels, step * kGroupNormMaxLanePixels);
+            if (k < least) k = least;
+            if (k < 1) k = 1;
+            p.chunk_pixels = gn_ceil(gn_ceil(pixels, k), step) * step;
+            p.chunks = (int)gn_ceil(pixels, p.chunk_pixels);
+            // what every workgroup of the second launch reads to have its groups' sums
+            if ((long long)p.chunks * p.slab_groups * 16 <= (32 << 10) || m == 1 || p.slab_vectors * p.vec * element_bytes <= 256) break;
+            m = (m + 1) / 2;
+        }
+        p.batch_blocks = batch;
+    }
+    const int lanes = p.slice_vectors * p.rows;
+    p.threads = (lanes + 63) / 64 * 64;
+    const size_t tree = (size_t)((p.rows + 1) / 2) * p.slice_vectors * p.vec * sizeof(double);
+    const size_t gather = (size_t)p.threads * 2 * sizeof(double);
+    p.lds_bytes = tree > gather ? tree : gather;
+    const long long samples = p.chunks > 1 ? batch : p.batch_blocks;
+    p.blocks = samples * p.slabs * p.chunks;
+    p.group_part_bytes = p.chunks > 1 ? (size_t)(batch * p.slabs * p.chunks) * p.slab_groups * 2 * sizeof(double) : 0;
+    p.channel_rows = backward ? samples * p.chunks : 0;
+    p.param_blocks = backward ? (int)gn_ceil(channels, kGroupNormParamChannels) : 0;
+    p.workspace_bytes = p.group_part_bytes + (size_t)p.channel_rows * 2 * channels * sizeof(float);
+    p.ok = p.blocks + p.param_blocks <= 0x7fffffffll && p.chunks >= 1 && p.lds_bytes <= (56u << 10);
+    return p;
+}
+
+struct GroupNormCall {
+    GroupNormPlan plan;
+    long long batch = 0, pixels = 0;
+    int channels = 0, groups = 0;
+    int type = 0;                   // GroupNormType of x, out, dout, dx
+    bool weight_fp32 = false;       // of weight, bias and their gradients; otherwise the arrays' type
+    int activation = 0;
+    float eps = 0;
+    const void* x = nullptr;
+    const void* dout = nullptr;     // backward
+    const void* weight = nullptr;   // null: 1
+    const void* bias = nullptr;     // null: 0
+    float* stats = nullptr;         // (batch, groups, 2): mean and 1/sqrt(var + eps); written forward, read backward
+    void* out = nullptr;            // y, or dx
+    void* dweight = nullptr;        // backward; may be null
+    void* dbias = nullptr;
+    void* workspace = nullptr;
+};
+
+// Enqueue the launches on `stream` of the current device; a hipError_t.
+int launch_group_norm_forward(const GroupNormCall& call, void* stream);
+int launch_group_norm_backward(const GroupNormCall& call, void* stream);
+
+}  // namespace sideaware

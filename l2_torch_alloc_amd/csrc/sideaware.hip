@@ -18,6 +18,7 @@
 #include <vector>
 
 #include "../../include/sideaware.h"
+#include "group_norm.h"
 #include "hip_backing.h"
 #include "launch_plan.h"
 #include "pool.h"
@@ -1203,6 +1204,98 @@ void sideaware_one_to_one(int kernel_id, size_t num_bytes, void* out0, const voi
 void sideaware_memcpy(void* out, const void* in, size_t num_bytes, int device, sideaware_stream_t stream) {
     sideaware_elementwise(0, num_bytes, out, nullptr, nullptr, nullptr, in, nullptr, nullptr, nullptr,
                           nullptr, 0, 0, 0, device, stream);
+}
+
+// ---- group norm -------------------------------------------------------------------------------
+
+static int group_norm_element_bytes(int dtype) {
+    return dtype == kGroupNormFp32 ? 4 : dtype == kGroupNormBf16 || dtype == kGroupNormFp16 ? 2 : 0;
+}
+
+// Null after recording what is wrong with the arguments.
+static DeviceContext* plan_group_norm_call(const char* what, long long batch, long long pixels, int channels, int groups, int dtype,
+                                           bool backward, int device, GroupNormPlan* plan) {
+    const int element = group_norm_element_bytes(dtype);
+    if (element == 0) {
+        set_error("%s: unknown type %d", what, dtype);
+        return nullptr;
+    }
+    if (batch < 1 || pixels < 1 || channels < 1 || groups < 1 || channels % groups) {
+        set_error("%s: %lld samples of %lld pixels, %d channels in %d groups: every count is at least 1 and the groups divide the channels",
+                  what, batch, pixels, channels, groups);
+        return nullptr;
+    }
+    if (batch > (1ll << 48) / pixels || batch * pixels > (1ll << 48) / channels) {
+        set_error("%s: %lld samples of %lld pixels of %d channels are too many", what, batch, pixels, channels);
+        return nullptr;
+    }
+    DeviceContext* ctx = get_context(device);
+    if (!ctx) return nullptr;
+    *plan = plan_group_norm(batch, pixels, channels, groups, element, backward, ctx->num_cus);
+    if (!plan->ok) {
+        set_error("%s: %lld samples of %lld pixels, %d channels in %d groups do not fit one launch", what, batch, pixels, channels, groups);
+        return nullptr;
+    }
+    return ctx;
+}
+
+size_t sideaware_group_norm_workspace(long long batch, long long pixels, int channels, int groups, int dtype, int backward, int device) {
+    GroupNormPlan plan;
+    return plan_group_norm_call("group_norm_workspace", batch, pixels, channels, groups, dtype, backward != 0, device, &plan)
+               ? plan.workspace_bytes : 0;
+}
+
+static int run_group_norm(const char* what, bool backward, GroupNormCall& call, int dtype, int weight_fp32, void* workspace, size_t workspace_bytes,
+                          int device, sideaware_stream_t stream) {
+    DeviceContext* ctx = plan_group_norm_call(what, call.batch, call.pixels, call.channels, call.groups, dtype, backward, device, &call.plan);
+    if (!ctx) return -1;
+    if (call.activation != kGroupNormNone && call.activation != kGroupNormSilu) {
+        set_error("%s: unknown activation %d", what, call.activation);
+        return -1;
+    }
+    if (!call.x || !call.out || !call.stats || (backward && !call.dout)) {
+        set_error("%s: null array", what);
+        return -1;
+    }
+    if (((uintptr_t)call.x | (uintptr_t)call.out | (uintptr_t)call.dout) % 16 || (uintptr_t)call.stats % 8 || (uintptr_t)workspace % 16) {
+        set_error("%s: arrays and workspace must start on multiples of 16 bytes (stats: 8)", what);
+        return -1;
+    }
+    if (workspace_bytes < call.plan.workspace_bytes || (call.plan.workspace_bytes && !workspace)) {
+        set_error("%s: the workspace has %zu of the %zu bytes needed", what, workspace ? workspace_bytes : 0, call.plan.workspace_bytes);
+        return -1;
+    }
+    call.type = dtype;
+    call.weight_fp32 = weight_fp32 != 0 || dtype == kGroupNormFp32;
+    call.workspace = workspace;
+    ScopedDevice guard(ctx->device);
+    const int err = backward ? launch_group_norm_backward(call, stream) : launch_group_norm_forward(call, stream);
+    if (err != (int)hipSuccess) {
+        set_error("%s: launch failed: %s", what, hipGetErrorString((hipError_t)err));
+        (void)hipGetLastError();
+    }
+    return err;
+}
+
+int sideaware_group_norm_forward(void* out, float* stats, const void* x, const void* weight, const void* bias,
+                                 long long batch, long long pixels, int channels, int groups, float eps, int activation,
+                                 int dtype, int weight_fp32, void* workspace, size_t workspace_bytes, int device, sideaware_stream_t stream) {
+    GroupNormCall call;
+    call.batch = batch; call.pixels = pixels; call.channels = channels; call.groups = groups;
+    call.activation = activation; call.eps = eps;
+    call.x = x; call.weight = weight; call.bias = bias; call.stats = stats; call.out = out;
+    return run_group_norm("group_norm_forward", false, call, dtype, weight_fp32, workspace, workspace_bytes, device, stream);
+}
+
+int sideaware_group_norm_backward(void* dx, void* dweight, void* dbias, const void* dout, const void* x, const void* weight, const void* bias,
+                                  const float* stats, long long batch, long long pixels, int channels, int groups, int activation,
+                                  int dtype, int weight_fp32, void* workspace, size_t workspace_bytes, int device, sideaware_stream_t stream) {
+    GroupNormCall call;
+    call.batch = batch; call.pixels = pixels; call.channels = channels; call.groups = groups;
+    call.activation = activation;
+    call.x = x; call.dout = dout; call.weight = weight; call.bias = bias; call.stats = (float*)stats; call.out = dx;
+    call.dweight = dweight; call.dbias = dbias;
+    return run_group_norm("group_norm_backward", true, call, dtype, weight_fp32, workspace, workspace_bytes, device, stream);
 }
 
 // ---- configuration ----------------------------------------------------------------------------

@@ -368,9 +368,7 @@ def _dropout(x: torch.Tensor, p: float, seed: torch.Tensor, residual: Optional[t
     if residual is not None:
         assert residual.shape == x.shape and residual.dtype == x.dtype and residual.device == x.device, \
             "the residual is like the activation"
-    if out is None:
-        out = torch.empty_like(x)
-    assert out.shape == x.shape and out.dtype == x.dtype and out.device == x.device, "the output is like the activation"
+    out = _like(out, x, "out")
     if x.numel():
         kid = _kernel("dropout", (dtype, residual is not None))
         _elementwise(kid, out, None, None, None, x, residual, None, None, seed, threshold, 0, 0)
@@ -390,6 +388,133 @@ def dropout_forward(x, p: float, seed, residual=None, out=None):
 def dropout_backward(dout, p: float, seed, out=None):
     """The gradient of :func:`dropout_forward` with respect to ``x`` (that of the residual is ``dout``)."""
     return _dropout(dout, p, seed, None, out)
+
+
+_GROUP_NORM_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_ACTIVATIONS = {"none": 0, "silu": 1}
+
+
+def _group_norm_shape(x: torch.Tensor, weight, bias, groups: int, activation: str):
+    """(batch, pixels, channels, type, weight_fp32, activation) of a call, checked."""
+    dtype = _GROUP_NORM_TYPES.get(x.dtype)
+    if dtype is None:
+        raise TypeError("group norm storage is float32, bfloat16 or float16")
+    if activation not in _ACTIVATIONS:
+        raise ValueError("the activation is 'none' or 'silu'")
+    assert x.dim() >= 2, "activations are (N, ..., C), channels last"
+    batch, channels = x.shape[0], x.shape[-1]
+    if groups < 1 or channels < 1 or channels % groups:
+        raise ValueError("%d groups do not divide %d channels" % (groups, channels))
+    pixels = x[0].numel() // channels if batch else 1
+    if pixels < 1:
+        raise ValueError("a sample without pixels has no mean")
+    params = [t for t in (weight, bias) if t is not None]
+    for t in params:
+        assert t.dtype in (torch.float32, x.dtype) and t.dtype == params[0].dtype, "weight and bias are both float32 or both of the activations' type"
+        assert tuple(t.shape) == (channels,) and t.is_contiguous() and t.device == x.device, \
+            "weight and bias have one value per channel, on the activations' device"
+    weight_fp32 = 1 if not params or params[0].dtype == torch.float32 else 0
+    return batch, pixels, channels, dtype, weight_fp32, _ACTIVATIONS[activation]
+
+
+def _may_allocate(what: str) -> None:
+    """Under this library's allocator, memory that is allocated while a stream is being captured goes back to
+    the pool when the tensor dies, while the graph still writes it."""
+    if wrapper._allocator_installed and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("under stream capture pass %s: the graph needs memory that outlives it" % what)
+
+
+def _like(t, x: torch.Tensor, name: str) -> torch.Tensor:
+    if t is None:
+        _may_allocate(name)
+        return torch.empty_like(x)
+    assert t.shape == x.shape and t.dtype == x.dtype and t.device == x.device, name + " is like the activation"
+    return t
+
+
+def _group_norm_workspace(workspace, batch, pixels, channels, groups, dtype, backward: bool, device: int):
+    need = wrapper.library().sideaware_group_norm_workspace(batch, pixels, channels, groups, dtype, int(backward), device)
+    if workspace is None:
+        if need == 0:
+            return 0, 0, None
+        _may_allocate("workspace")
+        workspace = torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", device))
+    assert workspace.is_cuda and workspace.get_device() == device and workspace.is_contiguous() and workspace.data_ptr() % 16 == 0, \
+        "the workspace is a contiguous tensor on the activations' device"
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
+
+
+def group_norm_workspace(x: torch.Tensor, groups: int, backward: bool = False) -> int:
+    """The bytes of ``workspace`` that :func:`group_norm_forward` (or backward) of ``x`` needs; may be 0."""
+    batch, pixels, channels, dtype, _, _ = _group_norm_shape(x, None, None, groups, "none")
+    if batch == 0:
+        return 0
+    return wrapper.library().sideaware_group_norm_workspace(batch, pixels, channels, groups, dtype, int(backward), x.get_device())
+
+
+def _group_norm_failed(what: str):
+    raise RuntimeError("%s: %s" % (what, wrapper.sideaware_last_error()))
+
+
+def group_norm_forward(x, weight, bias, groups: int, eps: float = 1e-5, activation: str = "none", out=None, stats=None, workspace=None):
+    """Group norm over (N, ..., C) activations, channels last: ``act((x - mean) / sqrt(var + eps) * weight + bias)``
+    with mean and variance over a sample's pixels and the C / groups channels of a group, and ``act`` either
+    "none" or "silu".  ``weight`` and ``bias`` are (C,), both float32 or both of x's type, or None.
+    Returns (y, stats), stats being float32 (N, groups, 2): mean and 1 / sqrt(var + eps), which
+    :func:`group_norm_backward` takes.  (A channels-last (N, C, H, W) tensor is ``t.permute(0, 2, 3, 1)``.)
+
+    ``out`` (may be ``x``), ``stats`` and ``workspace`` (:func:`group_norm_workspace` bytes, of any type) are
+    allocated unless given.  Under stream capture with this library's allocator they have to be given, and calls that can
+    overlap, such as two graphs' replays, each need their own."""
+    batch, pixels, channels, dtype, weight_fp32, act = _group_norm_shape(x, weight, bias, groups, activation)
+    out = _like(out, x, "out")
+    if stats is None:
+        _may_allocate("stats")
+        stats = torch.empty(batch, groups, 2, dtype=torch.float32, device=x.device)
+    assert tuple(stats.shape) == (batch, groups, 2) and stats.dtype == torch.float32 and stats.is_contiguous() and stats.device == x.device, \
+        "stats are float32 (N, groups, 2)"
+    if batch == 0:
+        return out, stats
+    x_ptr, out_ptr = wrapper._check(x, "x"), wrapper._check(out, "out")
+    device, stream = wrapper._device_and_stream(x)
+    ws_ptr, ws_bytes, keep = _group_norm_workspace(workspace, batch, pixels, channels, groups, dtype, False, device)
+    if wrapper.library().sideaware_group_norm_forward(
+            out_ptr, stats.data_ptr(), x_ptr, weight.data_ptr() if weight is not None else None, bias.data_ptr() if bias is not None else None,
+            batch, pixels, channels, groups, eps, act, dtype, weight_fp32, ws_ptr, ws_bytes, device, stream):
+        _group_norm_failed("group_norm_forward")
+    return out, stats
+
+
+def group_norm_backward(dout, x, weight, bias, stats, groups: int, activation: str = "none", out=None, dweight=None, dbias=None, workspace=None):
+    """The gradients of :func:`group_norm_forward`: (dx, dweight, dbias), the latter two of weight's type and summed
+    over samples and pixels (None where weight or bias is None).  ``stats`` is what the forward call returned.
+    ``out`` may be ``dout``.  ``out``, ``dweight``, ``dbias`` and ``workspace`` are allocated unless given, as for the
+    forward call."""
+    batch, pixels, channels, dtype, weight_fp32, act = _group_norm_shape(x, weight, bias, groups, activation)
+    assert dout.shape == x.shape and dout.dtype == x.dtype and dout.device == x.device, "the gradient is like the activation"
+    assert tuple(stats.shape) == (batch, groups, 2) and stats.dtype == torch.float32 and stats.is_contiguous() and stats.device == x.device, \
+        "stats are float32 (N, groups, 2)"
+    out = _like(out, x, "out")
+    grads = []
+    for given, param, name in ((dweight, weight, "dweight"), (dbias, bias, "dbias")):
+        assert given is None or param is not None, name + " goes with a parameter"
+        grads.append(None if param is None else _like(given, param, name))
+        assert param is None or grads[-1].is_contiguous(), name + " is contiguous"
+    dweight, dbias = grads
+    if batch == 0:
+        for t in grads:
+            if t is not None:
+                t.zero_()
+        return out, dweight, dbias
+    x_ptr, dout_ptr, out_ptr = wrapper._check(x, "x"), wrapper._check(dout, "dout"), wrapper._check(out, "out")
+    device, stream = wrapper._device_and_stream(x)
+    ws_ptr, ws_bytes, keep = _group_norm_workspace(workspace, batch, pixels, channels, groups, dtype, True, device)
+    if wrapper.library().sideaware_group_norm_backward(
+            out_ptr, dweight.data_ptr() if dweight is not None else None, dbias.data_ptr() if dbias is not None else None, dout_ptr, x_ptr,
+            weight.data_ptr() if weight is not None else None, bias.data_ptr() if bias is not None else None, stats.data_ptr(),
+            batch, pixels, channels, groups, act, dtype, weight_fp32, ws_ptr, ws_bytes, device, stream):
+        _group_norm_failed("group_norm_backward")
+    return out, dweight, dbias
 
 
 def scale_bias_bf16(x: torch.Tensor, scale_bias: torch.Tensor, out: Optional[torch.Tensor] = None):

@@ -32,7 +32,7 @@ _torch_side_index = None
 _gpu_side_index = None
 _cpu_side_index = None
 
-_vp, _ci, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t
+_vp, _ci, _sz, _ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_longlong
 
 # name -> (restype, argtypes).  Widths are those of include/sideaware.h.  Note the reference's
 # Python binding declares sideband_value as a pointer-sized integer (test.py:36); both widths
@@ -66,6 +66,9 @@ _SIGNATURES = {
     "sideaware_min_sm_per_side": (_ci, []),
     "sideaware_hash_mask": (_ci, []),
     "sideaware_elementwise_batch": (None, [_ci, _ci, _vp, _ci, _vp]),
+    "sideaware_group_norm_workspace": (_sz, [_ll, _ll, _ci, _ci, _ci, _ci, _ci]),
+    "sideaware_group_norm_forward": (_ci, [_vp, _vp, _vp, _vp, _vp, _ll, _ll, _ci, _ci, ctypes.c_float, _ci, _ci, _ci, _vp, _sz, _ci, _vp]),
+    "sideaware_group_norm_backward": (_ci, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _ll, _ci, _ci, _ci, _ci, _ci, _vp, _sz, _ci, _vp]),
     "sideaware_reserve_limit": (None, [_sz]),
     "sideaware_oom_raises": (None, [_ci]),
     "sideaware_arena_bytes": (None, [_sz]),

@@ -1,0 +1,62 @@
+// Reads "batch pixels channels groups element_bytes backward" lines and checks what the kernels rely on of
+// group_norm.h's plan: every (sample, pixel, channel) belongs to one workgroup and lane, groups are whole
+// inside slabs, and every workgroup's accesses to LDS and to the workspace stay inside what the plan asks for.
+#include <cstdio>
+#include <vector>
+
+#include "../../l2_torch_alloc_amd/csrc/group_norm.h"
+
+using namespace sideaware;
+
+#define REQUIRE(x) do { if (!(x)) { std::printf("FAIL %s: %s", #x, line); return 1; } } while (0)
+
+int main() {
+    char line[256];
+    long long batch, pixels;
+    int channels, groups, element, backward, cases = 0, one = 0;
+    while (std::fgets(line, sizeof line, stdin)) {
+        if (std::sscanf(line, "%lld %lld %d %d %d %d", &batch, &pixels, &channels, &groups, &element, &backward) != 6) continue;
+        cases++;
+        const GroupNormPlan p = plan_group_norm(batch, pixels, channels, groups, element, backward, 256);
+        REQUIRE(p.ok);
+        REQUIRE(p.vec >= 1 && p.vec * element <= 16 && channels % p.vec == 0 && p.row_vectors * p.vec == channels);
+        REQUIRE(p.group_channels * groups == channels);
+        // slabs: whole vectors, whole groups, all of the row
+        REQUIRE(p.slabs >= 1 && (long long)p.slabs * p.slab_vectors >= p.row_vectors && (long long)(p.slabs - 1) * p.slab_vectors < p.row_vectors);
+        REQUIRE(p.slab_vectors * p.vec == p.slab_groups * p.group_channels);
+        REQUIRE(p.slab_groups >= 1 && p.slab_groups <= kGroupNormMaxSlabGroups);
+        REQUIRE(p.slice_vectors >= 1 && p.slice_vectors <= kGroupNormMaxSlice && p.slice_vectors <= p.slab_vectors);
+        // lanes
+        REQUIRE(p.rows >= 1 && p.rows <= pixels && p.slice_vectors * p.rows <= p.threads);
+        REQUIRE(p.threads % 64 == 0 && p.threads >= 64 && p.threads <= kGroupNormMaxThreads);
+        // chunks: none empty, all pixels
+        REQUIRE(p.chunk_pixels >= 1 && p.chunks >= 1);
+        REQUIRE((p.chunks - 1) * p.chunk_pixels < pixels && p.chunks * p.chunk_pixels >= pixels);
+        REQUIRE((p.chunk_pixels + p.rows - 1) / p.rows <= kGroupNormMaxLanePixels);
+        // samples
+        const long long samples = p.chunks > 1 ? batch : p.batch_blocks;
+        REQUIRE(samples >= 1 && samples <= batch && p.blocks == samples * p.slabs * p.chunks);
+        REQUIRE(p.blocks + p.param_blocks <= 0x7fffffffll);
+        // LDS: the rows' tree, the channels of a slice, two doubles a thread
+        REQUIRE(p.lds_bytes >= (size_t)(p.rows - (p.rows + 1) / 2) * p.slice_vectors * p.vec * 8);
+        REQUIRE(p.lds_bytes >= (size_t)p.slice_vectors * p.vec * 8 && p.lds_bytes >= (size_t)p.threads * 16);
+        REQUIRE(p.lds_bytes + kGroupNormMaxSlabGroups * 24 <= 65536);
+        // workspace
+        if (p.chunks > 1) {
+            const long long last = (((batch - 1) * p.slabs + p.slabs - 1) * p.chunks + p.chunks - 1) * p.slab_groups * 2 + (p.slab_groups - 1) * 2 + 1;
+            REQUIRE((size_t)(last + 1) * 8 <= p.group_part_bytes);
+        } else {
+            REQUIRE(p.group_part_bytes == 0);
+            one++;
+        }
+        if (backward) {
+            REQUIRE(p.channel_rows == samples * p.chunks);
+            REQUIRE(p.workspace_bytes == p.group_part_bytes + (size_t)p.channel_rows * 2 * channels * 4);
+            REQUIRE((long long)p.param_blocks * kGroupNormParamChannels >= channels);
+        } else {
+            REQUIRE(p.workspace_bytes == p.group_part_bytes);
+        }
+    }
+    std::printf("cases=%d one_launch=%d ok\n", cases, one);
+    return 0;
+}
