@@ -5,8 +5,10 @@
 //   vector   `vec` channels of one pixel, 16 bytes at most: the widest power of two that divides the row
 //   slab     consecutive whole groups of channels, a whole number of vectors: one workgroup's share of a row
 //   slice    the part of a slab a workgroup walks at a time, one vector per lane (nearly always all of it)
-//   chunk    consecutive pixels of one sample: one workgroup's share of the pixels
-//   rows     pixels a workgroup works on side by side
+//   rows     pixels a workgroup works on side by side, next to each other
+//   chunk    one workgroup's share of a sample's pixels: of `chunks` runs of `rows` pixels, every chunk takes
+//            one, so that all workgroups together move through memory as one window (runs of their own for
+//            each, far apart, were half as fast)
 #pragma once
 
 #include <cstddef>
@@ -26,13 +28,15 @@ struct GroupNormPlan {
     int slice_vectors = 0;          // vectors of a slice: lanes side by side
     int rows = 1;
     int threads = 64;
-    long long chunk_pixels = 0;
     int chunks = 1;                 // per sample; 1: sums and application in one launch
     long long batch_blocks = 1;     // one launch: workgroups share out the samples of a slab, sample n to n % batch_blocks
     size_t lds_bytes = 0;
-    // workspace: doubles of the groups' sums [sample][slab][chunk][group of slab][2], then, backward,
-    // floats of the channels' sums [row][2][channel], a row for each (sample or batch block, chunk)
-    size_t group_part_bytes = 0;
+    // Chunks: whether a launch of its own adds up their sums, instead of every workgroup that applies them.
+    bool finish = false;
+    // workspace: doubles of the groups' sums [sample][slab][chunk][group of slab][2]; backward, with a launch
+    // that adds them up, floats of the groups' means [sample][group][2]; backward, floats of the channels' sums
+    // [row][2][channel], a row for each (sample or batch block, chunk)
+    size_t group_part_bytes = 0, means_bytes = 0;
     long long channel_rows = 0;
     size_t workspace_bytes = 0;
     long long blocks = 0;           // workgroups of a launch over the array
@@ -40,11 +44,19 @@ struct GroupNormPlan {
     bool ok = false;
 };
 
-constexpr int kGroupNormMaxThreads = 1024;
-constexpr int kGroupNormMaxSlice = 512;           // vectors: with 8 channels of doubles each, 32 KiB of LDS
+// Two workgroups of eight waves to a CU, which leaves each lane 128 registers.
+constexpr int kGroupNormMaxThreads = 512;
+constexpr int kGroupNormMaxSliceChannels = 1024;
 constexpr int kGroupNormMaxSlabGroups = 256;
 constexpr int kGroupNormParamChannels = 64;       // channels per workgroup that adds up their sums
 constexpr long long kGroupNormMaxLanePixels = 256;
+#ifndef GN_ONE
+#define GN_ONE (32 << 10)
+#define GN_GATHER (32 << 10)
+#endif
+constexpr long long kGroupNormOneLaunchBytes = GN_ONE;
+constexpr long long kGroupNormGatherBytes = GN_GATHER;
+constexpr long long kGroupNormMaxRowsBytes = 1ll << 30;    // a lane's offset among the rows has 32 bits
 
 inline long long gn_ceil(long long a, long long b) { return (a + b - 1) / b; }
 
@@ -61,13 +73,19 @@ inline GroupNormPlan plan_group_norm(long long batch, long long pixels, int chan
     while (unit % p.vec) unit += p.group_channels;
     const int unit_vectors = unit / p.vec, unit_groups = unit / p.group_channels, units = channels / unit;
 
+    const long long row_bytes = (long long)channels * element_bytes;
+    if (row_bytes > kGroupNormMaxRowsBytes || pixels > 0x7fffffffll) return p;
+
     auto cut = [&](int m) {                        // slabs of m units
         p.slab_vectors = m * unit_vectors;
         p.slab_groups = m * unit_groups;
         p.slabs = (int)gn_ceil(units, m);
-        p.slice_vectors = p.slab_vectors < kGroupNormMaxSlice ? p.slab_vectors : kGroupNormMaxSlice;
+        int most_slice = kGroupNormMaxSliceChannels / p.vec;
+        if (most_slice > kGroupNormMaxThreads) most_slice = kGroupNormMaxThreads;
+        p.slice_vectors = p.slab_vectors < most_slice ? p.slab_vectors : most_slice;
         const long long most_rows = kGroupNormMaxThreads / p.slice_vectors;
         p.rows = (int)(pixels < most_rows ? pixels : most_rows);
+        while (p.rows > 1 && p.rows * row_bytes > kGroupNormMaxRowsBytes) p.rows /= 2;
     };
     const int most_units = unit_groups * units <= kGroupNormMaxSlabGroups ? units : kGroupNormMaxSlabGroups / unit_groups;
 
@@ -75,48 +93,46 @@ inline GroupNormPlan plan_group_norm(long long batch, long long pixels, int chan
     // time out of its caches.  Else the pixels are cut into chunks as well, and a second launch applies
     // what the first one summed.
     const long long unit_bytes = pixels * unit_vectors * p.vec * element_bytes;
-    if (unit_bytes <= (128 << 10)) {
+    if (unit_bytes <= kGroupNormOneLaunchBytes) {
         int m = 1;
         // wider slabs while there are workgroups enough without, up to 512 bytes of a row
         while (2 * m <= most_units && 2 * m * unit_vectors <= 32 && batch * gn_ceil(units, 2 * m) >= 2 * num_cus &&
-               2 * m * unit_bytes <= (128 << 10))
+               2 * m * unit_bytes <= kGroupNormOneLaunchBytes)
             m *= 2;
         cut(m);
-        p.chunks = 1;
-        p.chunk_pixels = pixels;
         const long long want = gn_ceil(4ll * num_cus, p.slabs);
         p.batch_blocks = batch < want ? batch : want;
     } else {
-        int m = most_units;
-        while (true) {
-            cut(m);
+        {
+            cut(most_units);
             const long long step = p.rows;
-            const long long want = gn_ceil(2ll * num_cus, batch * p.slabs);
+            // as many workgroups as the device holds at once, and no second, half-empty turn
+            const long long want = 2ll * num_cus / (batch * p.slabs);
             long long most = gn_ceil(pixels, 4 * step);            // at least four pixels a lane
             if (most < 1) most = 1;
             long long k = want < most ? want : most;
             const long long least = gn_ceil(pixels, step * kGroupNormMaxLanePixels);
             if (k < least) k = least;
-            if (k < 1) k = 1;
-            p.chunk_pixels = gn_ceil(gn_ceil(pixels, k), step) * step;
-            p.chunks = (int)gn_ceil(pixels, p.chunk_pixels);
-            // what every workgroup of the second launch reads to have its groups' sums
-            if ((long long)p.chunks * p.slab_groups * 16 <= (32 << 10) || m == 1 || p.slab_vectors * p.vec * element_bytes <= 256) break;
-            m = (m + 1) / 2;
+            p.chunks = (int)(k < 1 ? 1 : k);
         }
+        p.finish = (long long)p.chunks * p.slab_groups * 16 > kGroupNormGatherBytes;
         p.batch_blocks = batch;
     }
     const int lanes = p.slice_vectors * p.rows;
     p.threads = (lanes + 63) / 64 * 64;
-    const size_t tree = (size_t)((p.rows + 1) / 2) * p.slice_vectors * p.vec * sizeof(double);
+    // forward: four doubles a lane.  backward: a float for each lane and channel, two doubles for each channel
+    // of the slice.  Either: two doubles a thread where the chunks' sums are added.
+    const size_t slice_channels = (size_t)p.slice_vectors * p.vec;
+    const size_t sums = backward ? p.rows * slice_channels * sizeof(float) + 2 * slice_channels * sizeof(double) + 8 : (size_t)lanes * 4 * sizeof(double);
     const size_t gather = (size_t)p.threads * 2 * sizeof(double);
-    p.lds_bytes = tree > gather ? tree : gather;
+    p.lds_bytes = sums > gather ? sums : gather;
     const long long samples = p.chunks > 1 ? batch : p.batch_blocks;
     p.blocks = samples * p.slabs * p.chunks;
     p.group_part_bytes = p.chunks > 1 ? (size_t)(batch * p.slabs * p.chunks) * p.slab_groups * 2 * sizeof(double) : 0;
     p.channel_rows = backward ? samples * p.chunks : 0;
     p.param_blocks = backward ? (int)gn_ceil(channels, kGroupNormParamChannels) : 0;
-    p.workspace_bytes = p.group_part_bytes + (size_t)p.channel_rows * 2 * channels * sizeof(float);
+    p.means_bytes = backward && p.finish ? ((size_t)batch * groups * 2 * sizeof(float) + 15) / 16 * 16 : 0;
+    p.workspace_bytes = p.group_part_bytes + p.means_bytes + (size_t)p.channel_rows * 2 * channels * sizeof(float);
     p.ok = p.blocks + p.param_blocks <= 0x7fffffffll && p.chunks >= 1 && p.lds_bytes <= (56u << 10);
     return p;
 }

@@ -25,33 +25,37 @@ int main() {
         REQUIRE(p.slabs >= 1 && (long long)p.slabs * p.slab_vectors >= p.row_vectors && (long long)(p.slabs - 1) * p.slab_vectors < p.row_vectors);
         REQUIRE(p.slab_vectors * p.vec == p.slab_groups * p.group_channels);
         REQUIRE(p.slab_groups >= 1 && p.slab_groups <= kGroupNormMaxSlabGroups);
-        REQUIRE(p.slice_vectors >= 1 && p.slice_vectors <= kGroupNormMaxSlice && p.slice_vectors <= p.slab_vectors);
+        REQUIRE(p.slice_vectors >= 1 && p.slice_vectors * p.vec <= kGroupNormMaxSliceChannels && p.slice_vectors <= p.slab_vectors);
         // lanes
         REQUIRE(p.rows >= 1 && p.rows <= pixels && p.slice_vectors * p.rows <= p.threads);
         REQUIRE(p.threads % 64 == 0 && p.threads >= 64 && p.threads <= kGroupNormMaxThreads);
-        // chunks: none empty, all pixels
-        REQUIRE(p.chunk_pixels >= 1 && p.chunks >= 1);
-        REQUIRE((p.chunks - 1) * p.chunk_pixels < pixels && p.chunks * p.chunk_pixels >= pixels);
-        REQUIRE((p.chunk_pixels + p.rows - 1) / p.rows <= kGroupNormMaxLanePixels);
+        // chunks: none empty, none with more pixels to a lane than its sums may hold
+        REQUIRE(p.chunks >= 1 && (long long)(p.chunks - 1) * p.rows < pixels && (long long)p.chunks * p.rows < (1ll << 32));
+        REQUIRE((pixels + (long long)p.chunks * p.rows - 1) / ((long long)p.chunks * p.rows) <= kGroupNormMaxLanePixels);
+        REQUIRE((long long)p.rows * channels * element <= kGroupNormMaxRowsBytes);
         // samples
         const long long samples = p.chunks > 1 ? batch : p.batch_blocks;
         REQUIRE(samples >= 1 && samples <= batch && p.blocks == samples * p.slabs * p.chunks);
         REQUIRE(p.blocks + p.param_blocks <= 0x7fffffffll);
-        // LDS: the rows' tree, the channels of a slice, two doubles a thread
-        REQUIRE(p.lds_bytes >= (size_t)(p.rows - (p.rows + 1) / 2) * p.slice_vectors * p.vec * 8);
-        REQUIRE(p.lds_bytes >= (size_t)p.slice_vectors * p.vec * 8 && p.lds_bytes >= (size_t)p.threads * 16);
+        // LDS: forward four doubles a lane; backward a float for each lane's channel, rounded up to a double, and two
+        // doubles for each channel of the slice; two doubles a thread
+        const size_t slice_channels = (size_t)p.slice_vectors * p.vec;
+        if (backward) REQUIRE(p.lds_bytes >= (p.rows * slice_channels + 1) / 2 * 8 + 2 * slice_channels * 8);
+        else REQUIRE(p.lds_bytes >= (size_t)p.slice_vectors * p.rows * 32);
+        REQUIRE(p.lds_bytes >= (size_t)p.threads * 16);
         REQUIRE(p.lds_bytes + kGroupNormMaxSlabGroups * 24 <= 65536);
         // workspace
         if (p.chunks > 1) {
             const long long last = (((batch - 1) * p.slabs + p.slabs - 1) * p.chunks + p.chunks - 1) * p.slab_groups * 2 + (p.slab_groups - 1) * 2 + 1;
             REQUIRE((size_t)(last + 1) * 8 <= p.group_part_bytes);
+            if (p.finish && backward) REQUIRE(p.means_bytes >= (size_t)batch * groups * 8 && p.means_bytes % 16 == 0);
         } else {
             REQUIRE(p.group_part_bytes == 0);
             one++;
         }
         if (backward) {
             REQUIRE(p.channel_rows == samples * p.chunks);
-            REQUIRE(p.workspace_bytes == p.group_part_bytes + (size_t)p.channel_rows * 2 * channels * 4);
+            REQUIRE(p.workspace_bytes == p.group_part_bytes + p.means_bytes + (size_t)p.channel_rows * 2 * channels * 4);
             REQUIRE((long long)p.param_blocks * kGroupNormParamChannels >= channels);
         } else {
             REQUIRE(p.workspace_bytes == p.group_part_bytes);

@@ -35,14 +35,14 @@ def grouped(a, G):
 
 
 def check_forward(y, stats, x, w, b, G, eps, activation):
-    """Tolerances.  A lane's sums of d = x - pivot and d^2 over at most L pixels are off by L u of the sums of the
-    magnitudes, and |d| <= 2 D where D is the largest |x - mean| of the group; the mean is off by that and by its
+    """Tolerances.  A lane's sums of d = x - pivot and d^2 over at most 256 pixels and then the 8 channels of a vector,
+    L = 264 at most, are off by L u of the sums of the magnitudes, and |d| <= 2 D where D is the largest |x - mean| of the group; the mean is off by that and by its
     rounding, the variance by (L + 4) u (2 D)^2 / var of itself, 1/sqrt of it by half as much."""
     X, W, B = f64(x), 1.0 if w is None else f64(w), 0.0 if b is None else f64(b)
     N, P, C = X.shape
     want, want_stats = S.group_norm(X, W, B, G, float(np.float32(eps)), activation)
     mean, rstd = want_stats[..., 0], want_stats[..., 1]
-    L = min(P, 256)
+    L = min(P, 256) + 8
     D = np.abs(grouped(X, G) - mean[:, None, :, None]).max((1, 3))
     e_mean = U * np.abs(mean) + L * U * 2 * D
     e_rstd = rstd * ((L / 2 + 4) * U * (2 * D * rstd) ** 2 + 4 * U)
