@@ -39,7 +39,8 @@ struct GroupNormPlan {
     size_t group_part_bytes = 0, means_bytes = 0;
     long long channel_rows = 0;
     size_t workspace_bytes = 0;
-    long long blocks = 0;           // workgroups of a launch over the array
+    bool stream = false;            // the arrays do not fit the Infinity Cache together
+    long long blocks = 0;           // workgroups of a launch over the array: chunks x slabs x batch_blocks
     int param_blocks = 0;           // workgroups that add up the channels' sums
     bool ok = false;
 };
@@ -48,20 +49,17 @@ struct GroupNormPlan {
 constexpr int kGroupNormMaxThreads = 512;
 constexpr int kGroupNormMaxSliceChannels = 1024;
 constexpr int kGroupNormMaxSlabGroups = 256;
-constexpr int kGroupNormParamChannels = 64;       // channels per workgroup that adds up their sums
+constexpr int kGroupNormParamChannels = 16;       // channels per workgroup that adds up their sums
 constexpr long long kGroupNormMaxLanePixels = 256;
-#ifndef GN_ONE
-#define GN_ONE (32 << 10)
-#define GN_GATHER (32 << 10)
-#endif
-constexpr long long kGroupNormOneLaunchBytes = GN_ONE;
-constexpr long long kGroupNormGatherBytes = GN_GATHER;
+constexpr long long kGroupNormOneLaunchBytes = 32 << 10;
+constexpr long long kGroupNormGatherBytes = 64 << 10;
+constexpr long long kGroupNormMaxGrid = 65535;            // of the second and third axis
 constexpr long long kGroupNormMaxRowsBytes = 1ll << 30;    // a lane's offset among the rows has 32 bits
 
 inline long long gn_ceil(long long a, long long b) { return (a + b - 1) / b; }
 
 inline GroupNormPlan plan_group_norm(long long batch, long long pixels, int channels, int groups, int element_bytes, bool backward,
-                                     int num_cus) {
+                                     int num_cus, long long cache_bytes = 256ll << 20) {
     GroupNormPlan p;
     if (batch < 1 || pixels < 1 || channels < 1 || groups < 1 || channels % groups || num_cus < 1) return p;
     p.vec = 16 / element_bytes;
@@ -76,18 +74,21 @@ inline GroupNormPlan plan_group_norm(long long batch, long long pixels, int chan
     const long long row_bytes = (long long)channels * element_bytes;
     if (row_bytes > kGroupNormMaxRowsBytes || pixels > 0x7fffffffll) return p;
 
+    int most_slice = kGroupNormMaxSliceChannels / p.vec;
+    if (most_slice > kGroupNormMaxThreads) most_slice = kGroupNormMaxThreads;
     auto cut = [&](int m) {                        // slabs of m units
         p.slab_vectors = m * unit_vectors;
         p.slab_groups = m * unit_groups;
         p.slabs = (int)gn_ceil(units, m);
-        int most_slice = kGroupNormMaxSliceChannels / p.vec;
-        if (most_slice > kGroupNormMaxThreads) most_slice = kGroupNormMaxThreads;
         p.slice_vectors = p.slab_vectors < most_slice ? p.slab_vectors : most_slice;
         const long long most_rows = kGroupNormMaxThreads / p.slice_vectors;
         p.rows = (int)(pixels < most_rows ? pixels : most_rows);
         while (p.rows > 1 && p.rows * row_bytes > kGroupNormMaxRowsBytes) p.rows /= 2;
     };
-    const int most_units = unit_groups * units <= kGroupNormMaxSlabGroups ? units : kGroupNormMaxSlabGroups / unit_groups;
+    // the widest slabs: of one slice, if a unit is not wider; all of about the same width
+    int most_units = kGroupNormMaxSlabGroups / unit_groups;
+    if (most_units > most_slice / unit_vectors) most_units = most_slice / unit_vectors > 1 ? most_slice / unit_vectors : 1;
+    most_units = (int)gn_ceil(units, gn_ceil(units, most_units));
 
     // One launch where a sample's part of the smallest slab is little: a workgroup then reads it a second
     // time out of its caches.  Else the pixels are cut into chunks as well, and a second launch applies
@@ -103,37 +104,35 @@ inline GroupNormPlan plan_group_norm(long long batch, long long pixels, int chan
         const long long want = gn_ceil(4ll * num_cus, p.slabs);
         p.batch_blocks = batch < want ? batch : want;
     } else {
-        {
-            cut(most_units);
-            const long long step = p.rows;
-            // as many workgroups as the device holds at once, and no second, half-empty turn
-            const long long want = 2ll * num_cus / (batch * p.slabs);
-            long long most = gn_ceil(pixels, 4 * step);            // at least four pixels a lane
-            if (most < 1) most = 1;
-            long long k = want < most ? want : most;
-            const long long least = gn_ceil(pixels, step * kGroupNormMaxLanePixels);
-            if (k < least) k = least;
-            p.chunks = (int)(k < 1 ? 1 : k);
-        }
+        cut(most_units);
+        const long long step = p.rows;
+        // as many workgroups as the device holds at once, and no second, half-empty turn; at least four pixels a lane
+        const long long want = 2ll * num_cus / (batch * p.slabs), most = gn_ceil(pixels, 4 * step);
+        const long long least = gn_ceil(pixels, step * kGroupNormMaxLanePixels);
+        long long k = want < most ? want : most;
+        if (k < least) k = least;
+        p.chunks = (int)(k < 1 ? 1 : k);
         p.finish = (long long)p.chunks * p.slab_groups * 16 > kGroupNormGatherBytes;
-        p.batch_blocks = batch;
+        p.batch_blocks = batch < kGroupNormMaxGrid ? batch : kGroupNormMaxGrid;
     }
+    p.stream = batch * pixels * row_bytes * (backward ? 3 : 2) > cache_bytes / 4 * 3;
     const int lanes = p.slice_vectors * p.rows;
     p.threads = (lanes + 63) / 64 * 64;
-    // forward: four doubles a lane.  backward: a float for each lane and channel, two doubles for each channel
+    // forward: four doubles a lane.  backward: two floats for each lane and channel, two doubles for each channel
     // of the slice.  Either: two doubles a thread where the chunks' sums are added.
     const size_t slice_channels = (size_t)p.slice_vectors * p.vec;
-    const size_t sums = backward ? p.rows * slice_channels * sizeof(float) + 2 * slice_channels * sizeof(double) + 8 : (size_t)lanes * 4 * sizeof(double);
+    const size_t sums = backward ? p.rows * slice_channels * 2 * sizeof(float) + slice_channels * 2 * sizeof(double) : (size_t)lanes * 4 * sizeof(double);
     const size_t gather = (size_t)p.threads * 2 * sizeof(double);
     p.lds_bytes = sums > gather ? sums : gather;
-    const long long samples = p.chunks > 1 ? batch : p.batch_blocks;
-    p.blocks = samples * p.slabs * p.chunks;
+    p.blocks = p.batch_blocks * p.slabs * p.chunks;
     p.group_part_bytes = p.chunks > 1 ? (size_t)(batch * p.slabs * p.chunks) * p.slab_groups * 2 * sizeof(double) : 0;
-    p.channel_rows = backward ? samples * p.chunks : 0;
+    p.channel_rows = backward ? p.batch_blocks * p.chunks : 0;
     p.param_blocks = backward ? (int)gn_ceil(channels, kGroupNormParamChannels) : 0;
     p.means_bytes = backward && p.finish ? ((size_t)batch * groups * 2 * sizeof(float) + 15) / 16 * 16 : 0;
     p.workspace_bytes = p.group_part_bytes + p.means_bytes + (size_t)p.channel_rows * 2 * channels * sizeof(float);
-    p.ok = p.blocks + p.param_blocks <= 0x7fffffffll && p.chunks >= 1 && p.lds_bytes <= (56u << 10);
+    // the workgroups that add up the parameters' gradients widen the first axis, for each of the others
+    const long long others = p.slabs * p.batch_blocks;
+    p.ok = p.slabs <= kGroupNormMaxGrid && (p.chunks + gn_ceil(p.param_blocks, others)) * others <= 0x7fffffffll && p.lds_bytes <= (56u << 10);
     return p;
 }
 

@@ -33,12 +33,19 @@ struct GnArgs {
     double* group_part;
     float* means;
     float* channel_part;
-    long long batch, pixels, batch_blocks, channel_rows, main_blocks;
+    long long batch, pixels, channel_rows;
     double inv_count;               // 1 / (pixels * channels of a group)
-    int channels, groups, group_channels, row_vectors;
-    int slab_vectors, slabs, slab_groups, slice_vectors, rows, chunks;
-    int weight_fp32, activation, finish;
+    float inv_group_channels;
     float eps;
+    unsigned int inv_slice, inv_gather;      // 2^20 / slice_vectors and / gather_groups, rounded up: for thread numbers below 512
+    int channels, groups, group_channels, row_vectors;
+    int slab_vectors, slab_groups, slice_vectors, rows, chunks;
+    int runs, more_runs;            // runs of pixels of every chunk; the first `more_runs` chunks have one more
+    int last_chunk, last_pixels;    // the chunk whose last run is not whole, and its pixels; -1 and 0: all are whole
+    int gather_groups, gather_threads;       // groups whose chunks' sums are added at once, and threads to each
+    int per_group_log2;             // threads to a group where lanes' sums are added
+    int param_x, param_blocks;      // workgroups of a row of the grid that add up dw and db, and how many do in all
+    int weight_fp32, activation, finish;
 };
 
 // The values of a vector stay packed in whole words until they are used: as an array of 16-bit values each of
@@ -66,6 +73,24 @@ struct Vec {
         __builtin_memcpy(&words, v, sizeof words);
     }
 };
+
+// Stores are written through the private L2 (`sc1`), which spares the end of the launch the write-backs: 22.2 us against
+// 24.1 for 8 images of 64x64 pixels of 320 bf16 channels.  Where the arrays together exceed the Infinity Cache the
+// output is not kept there either (`nt`): what the next call reads then does not wait for this one's output to be
+// written back (512x512 pixels of 256 channels: 78 us against 88).  Narrow vectors are left to the L2, which may merge them.
+// The two wait states: hardware reads the data registers of a store wider than 8 bytes for two more issue cycles, and the
+// compiler does not look inside the statement.
+template<bool STREAM, typename W>
+__device__ __forceinline__ void store_words(void* to, const W& words) {
+    if constexpr (sizeof(W) == 16) {
+        if constexpr (STREAM) asm volatile("global_store_dwordx4 %0, %1, off sc1 nt\n\ts_nop 1" : : "v"(to), "v"(words) : "memory");
+        else asm volatile("global_store_dwordx4 %0, %1, off sc1\n\ts_nop 1" : : "v"(to), "v"(words) : "memory");
+    } else if constexpr (STREAM) {
+        __builtin_nontemporal_store(words, (W*)to);
+    } else {
+        *(W*)to = words;
+    }
+}
 
 // One parameter (weight or bias) of each of a lane's channels.  The vector may start anywhere a value may.
 template<typename T, int VEC>
@@ -104,26 +129,17 @@ struct Place {
     int tx, ty;
 };
 
-__device__ __forceinline__ Place place_of(const GnArgs& a, unsigned int block) {
+// The grid is (chunks, slabs, samples), so nothing is divided here.
+__device__ __forceinline__ Place place_of(const GnArgs& a, int chunk) {
     Place q;
-    unsigned int rest = block;
-    q.chunk = 0;
-    if (a.chunks > 1) {
-        rest = block / (unsigned int)a.chunks;
-        q.chunk = (int)(block - rest * (unsigned int)a.chunks);
-    }
-    unsigned int n = rest;
-    q.slab = 0;
-    if (a.slabs > 1) {
-        n = rest / (unsigned int)a.slabs;
-        q.slab = (int)(rest - n * (unsigned int)a.slabs);
-    }
-    q.n = n;
+    q.chunk = chunk;
+    q.slab = (int)blockIdx.y;
+    q.n = blockIdx.z;
     q.first_vector = q.slab * a.slab_vectors;
     q.end_vector = min(q.first_vector + a.slab_vectors, a.row_vectors);
     q.first_group = q.slab * a.slab_groups;
     q.groups = min(a.slab_groups, a.groups - q.first_group);
-    q.ty = (int)threadIdx.x / a.slice_vectors;
+    q.ty = (int)((threadIdx.x * a.inv_slice) >> 20);
     q.tx = (int)threadIdx.x - q.ty * a.slice_vectors;
     return q;
 }
@@ -140,96 +156,107 @@ struct Lane {
     int count = 0;                  // the lane's pixels; 0: it has none
     int v;                          // vector of the row
     __device__ __forceinline__ Lane(const GnArgs& a, const Place& q, long long n, int v0) {
-        const unsigned int stride = (unsigned int)a.chunks * (unsigned int)a.rows;
-        const unsigned int first = (unsigned int)q.chunk * (unsigned int)a.rows;
-        const unsigned int left = (unsigned int)a.pixels - first;
-        whole = (int)(left / stride);
-        unsigned int more = left - (unsigned int)whole * stride;         // pixels from the start of the last run
-        runs = whole + (more > 0 ? 1 : 0);
-        if (more >= (unsigned int)a.rows) { whole++; more = 0; }
+        runs = a.runs + (q.chunk < a.more_runs ? 1 : 0);
+        whole = q.chunk == a.last_chunk ? runs - 1 : runs;
         v = v0 + q.tx;
-        base = (n * a.pixels + first) * a.row_vectors * (long long)sizeof(V);
-        step = (long long)stride * a.row_vectors * (long long)sizeof(V);
+        const long long vector = sizeof(V);
+        base = (n * a.pixels + (long long)q.chunk * a.rows) * a.row_vectors * vector;
+        step = (long long)a.chunks * a.rows * a.row_vectors * vector;
         off = (unsigned int)(q.ty * a.row_vectors + v) * (unsigned int)sizeof(V);
-        const bool in_last = whole == runs || (unsigned int)q.ty < more;
+        const bool in_last = whole == runs || q.ty < a.last_pixels;
         off_last = in_last ? off : (unsigned int)v * (unsigned int)sizeof(V);
-        if (q.ty < a.rows && v < min(v0 + a.slice_vectors, q.end_vector)) count = whole == runs || in_last ? runs : whole;
+        if (q.ty < a.rows && v < min(v0 + a.slice_vectors, q.end_vector)) count = in_last ? runs : whole;
     }
     // B pixels from the i-th run on; behind the last one, and where the lane has none, some other, so that all
     // loads are made side by side with nothing to wait for in between
-    template<bool NT = false, int B>
+    template<int B>
     __device__ __forceinline__ void load(V (&to)[B], const void* array, int i) const {
         #pragma unroll
-        for (int u = 0; u < B; u++) to[u] = load<NT>(array, min(i + u, runs - 1));
+        for (int u = 0; u < B; u++) to[u] = load(array, min(i + u, runs - 1));
     }
-    template<bool NT = false>
     __device__ __forceinline__ V load(const void* array, int run) const {
-        const auto* from = (const decltype(V::words)*)((const char*)array + base + run * step + (run < whole ? off : off_last));
-        V to;
-        to.words = NT ? __builtin_nontemporal_load(from) : *from;
-        return to;
+        return *(const V*)((const char*)array + base + run * step + (run < whole ? off : off_last));
     }
+    template<bool STREAM>
     __device__ __forceinline__ void store(void* array, int i, const V& value) const {
-        auto* to = (decltype(V::words)*)((char*)array + base + i * step + off);
-#ifndef GN_ST
-#define GN_ST 0
-#endif
-        if constexpr (GN_ST == 1 || (GN_ST >= 2 && sizeof(value.words) < 16)) __builtin_nontemporal_store(value.words, to);
-        else if constexpr (GN_ST == 2) { auto w = value.words; asm volatile("global_store_dwordx4 %0, %1, off sc1\n\ts_nop 1" : : "v"(to), "v"(w) : "memory"); }
-        else if constexpr (GN_ST == 3) { auto w = value.words; asm volatile("global_store_dwordx4 %0, %1, off sc1 nt\n\ts_nop 1" : : "v"(to), "v"(w) : "memory"); }
-        else *to = value.words;
+        store_words<STREAM>((char*)array + base + i * step + off, value.words);
     }
 };
 
-// The slab's group (counted from its first) of each channel of a vector.
+// The slab's group of its channel c: by a reciprocal, which is off by one at most.
+__device__ __forceinline__ int group_of(const GnArgs& a, int c) {
+    int g = (int)((float)c * a.inv_group_channels);
+    if (g * a.group_channels > c) g--;
+    if ((g + 1) * a.group_channels <= c) g++;
+    return g;
+}
+
+// The slab's group of each channel of a vector.
 template<int VEC>
 __device__ __forceinline__ void groups_of(int (&g)[VEC], const GnArgs& a, const Place& q, int v) {
-    int at = v * VEC / a.group_channels, left = (at + 1) * a.group_channels - v * VEC;
+    const int c = (v - q.first_vector) * VEC;
+    int at = group_of(a, c), left = (at + 1) * a.group_channels - c;
     #pragma unroll
     for (int j = 0; j < VEC; j++) {
-        g[j] = at - q.first_group;
+        g[j] = at;
         if (--left == 0) { at++; left = a.group_channels; }
     }
 }
 
-// Threads that share one of `groups` sums: a power of two, in one wave.
-__device__ __forceinline__ int threads_per_group(int groups) {
-    int per = 1;
-    while (per < 64 && per * 2 * groups <= (int)blockDim.x) per *= 2;
-    return per;
+template<int CTRL>
+__device__ __forceinline__ double moved(double t) {
+    return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(t), CTRL, 0xf, 0xf, false),
+                            __builtin_amdgcn_update_dpp(0, __double2loint(t), CTRL, 0xf, 0xf, false));
 }
 
-__device__ __forceinline__ double add_over(double t, int per) {
-    for (int d = per / 2; d > 0; d /= 2) t += __shfl_xor(t, d, 64);
+// The sum over 2^per_log2 neighbouring threads of a wave, to all of them: moves inside a row of 16 lanes run in the
+// vector ALU.
+__device__ __forceinline__ double add_over(double t, int per_log2) {
+    if (per_log2 > 0) t += moved<0xB1>(t);                        // quad_perm [1,0,3,2]
+    if (per_log2 > 1) t += moved<0x4E>(t);                        // quad_perm [2,3,0,1]
+    if (per_log2 > 2) t += moved<0x141>(t);                       // row_half_mirror: the other quad, all of it alike
+    if (per_log2 > 3) t += moved<0x140>(t);                       // row_mirror: the other half of the row
+    if (per_log2 > 4) t += __shfl_xor(t, 16, 64);
+    if (per_log2 > 5) t += __shfl_xor(t, 32, 64);
     return t;
 }
 
 // The sums of the chunks of a sample's slab, by the workgroup of any chunk: sums[group] = {S1, S2}.
-__device__ __forceinline__ void gather_chunks(const GnArgs& a, const Place& q, double* lds, double (*sums)[2]) {
-    const double* part = a.group_part + (q.n * a.slabs + q.slab) * a.chunks * a.slab_groups * 2;
-    for (int base = 0; base < q.groups; base += (int)blockDim.x) {
-        const int here = min(q.groups - base, (int)blockDim.x);
-        const int per = (int)blockDim.x / here;                   // threads that share a group's chunks
-        const int g = (int)threadIdx.x % here, part_of = (int)threadIdx.x / here;
-        double s1 = 0, s2 = 0;
-        if (part_of < per) {
-            for (int k = part_of; k < a.chunks; k += per) {
-                const double* at = part + ((long long)k * a.slab_groups + base + g) * 2;
-                s1 += at[0];
-                s2 += at[1];
+__device__ __forceinline__ void gather_chunks(const GnArgs& a, const Place& q, long long n, double* lds, double (*sums)[2]) {
+    const double2* part = (const double2*)a.group_part + (n * gridDim.y + q.slab) * a.chunks * a.slab_groups;
+    double2* lanes = (double2*)lds;
+    const int share = (int)((threadIdx.x * a.inv_gather) >> 20), in = (int)threadIdx.x - share * a.gather_groups;
+    for (int base = 0; base < q.groups; base += a.gather_groups) {
+        const int g = base + in;
+        if (share < a.gather_threads) {
+            double2 t = {0, 0};
+            if (g < q.groups) {
+                // eight at a time, so that they are waited for once
+                for (int k = share; k < a.chunks; k += 8 * a.gather_threads) {
+                    double2 in4[8];
+                    #pragma unroll
+                    for (int u = 0; u < 8; u++) in4[u] = part[(long long)min(k + u * a.gather_threads, a.chunks - 1) * a.slab_groups + g];
+                    #pragma unroll
+                    for (int u = 0; u < 8; u++) {
+                        const bool on = k + u * a.gather_threads < a.chunks;
+                        t.x += on ? in4[u].x : 0.0;
+                        t.y += on ? in4[u].y : 0.0;
+                    }
+                }
             }
-            lds[threadIdx.x * 2] = s1;
-            lds[threadIdx.x * 2 + 1] = s2;
+            lanes[threadIdx.x] = t;
         }
         __syncthreads();
-        if ((int)threadIdx.x < here) {
-            s1 = s2 = 0;
-            for (int i = 0; i < per; i++) {
-                s1 += lds[(i * here + g) * 2];
-                s2 += lds[(i * here + g) * 2 + 1];
+        if ((int)threadIdx.x < a.gather_groups && g < q.groups) {
+            double2 t = {0, 0};
+            #pragma unroll 4
+            for (int i = 0; i < a.gather_threads; i++) {
+                const double2 more = lanes[i * a.gather_groups + in];
+                t.x += more.x;
+                t.y += more.y;
             }
-            sums[base + g][0] = s1;
-            sums[base + g][1] = s2;
+            sums[g][0] = t.x;
+            sums[g][1] = t.y;
         }
         __syncthreads();
     }
@@ -240,15 +267,17 @@ __device__ __forceinline__ void clear_sums(const Place& q, double (*sums)[2]) {
     __syncthreads();
 }
 
-__device__ __forceinline__ void write_part(const GnArgs& a, const Place& q, double (*sums)[2]) {
-    double* part = a.group_part + ((q.n * a.slabs + q.slab) * a.chunks + q.chunk) * a.slab_groups * 2;
+__device__ __forceinline__ void write_part(const GnArgs& a, const Place& q, long long n, double (*sums)[2]) {
+    double* part = a.group_part + ((n * gridDim.y + q.slab) * a.chunks + q.chunk) * a.slab_groups * 2;
     for (int g = (int)threadIdx.x; g < q.groups; g += (int)blockDim.x) {
         part[g * 2] = sums[g][0];
         part[g * 2 + 1] = sums[g][1];
     }
 }
 
-enum Mode { kSums, kApply, kBoth };
+// kApplyStream: as kApply, where the arrays exceed the Infinity Cache.
+enum Mode { kSums, kApply, kApplyStream, kBoth };
+constexpr bool applies_only(int mode) { return mode == kApply || mode == kApplyStream; }
 
 // All workgroups start together and would stay in step: every lane waiting for its batch of loads, then every lane
 // computing and the memory idle.  So the load that follows on a pixel's heels is issued where that pixel's registers are
@@ -258,7 +287,7 @@ __device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); 
 // ---- forward -----------------------------------------------------------------------------------
 
 // Pixels whose loads a lane has in flight: as many as fit its registers without spilling.
-constexpr int forward_batch(int mode) { return mode == kApply ? 4 : 6; }
+constexpr int forward_batch(int mode) { return applies_only(mode) ? 3 : 4; }
 
 // The sums of d = x - pivot and of d^2 over the lane's pixels, by channel.  The pivot is the lane's first
 // value of the group a channel belongs to.
@@ -284,6 +313,7 @@ __device__ __forceinline__ void forward_lane_sums(const GnArgs& a, const Lane<T,
         }
     };
     int i = 0;
+    #pragma unroll 1
     for (; i + 2 * B <= lane.whole; i += B) {
         #pragma unroll
         for (int u = 0; u < B; u++) {
@@ -292,19 +322,15 @@ __device__ __forceinline__ void forward_lane_sums(const GnArgs& a, const Lane<T,
             in_order();
         }
     }
-    #pragma unroll
-    for (int u = 0; u < B; u++) {
-        if (i + u < lane.count) add(cur[u]);
-        if (i + B + u < lane.runs) {
-            cur[u] = lane.load(a.x, i + B + u);
+    #pragma unroll 1
+    for (; i < lane.runs; i += B) {
+        #pragma unroll
+        for (int u = 0; u < B; u++) {
+            if (i + u < lane.count) add(cur[u]);
+            if (i + B + u < lane.runs) {
+                cur[u] = lane.load(a.x, i + B + u);
+            }
         }
-        in_order();
-    }
-    i += B;
-    if (i >= lane.runs) return;
-    #pragma unroll
-    for (int u = 0; u < B; u++) {
-        if (i + u < lane.count) add(cur[u]);
     }
 }
 
@@ -315,9 +341,9 @@ template<int VEC>
 __device__ __forceinline__ void forward_group_sums(const GnArgs& a, const Place& q, int v0, int count, const int (&g)[VEC], const float (&pivot)[VEC],
                                                    const float (&s1)[VEC], const float (&s2)[VEC], double* lds, double (*sums)[2]) {
     const int passes = a.group_channels >= VEC ? 1 : (VEC / a.group_channels + 2) / 2;
-    const int end = min(v0 + a.slice_vectors, q.end_vector);
-    const int per = threads_per_group(q.groups);
-    const int first = (int)threadIdx.x / per, part = (int)threadIdx.x % per, step = (int)blockDim.x / per;
+    const int end = min(v0 + a.slice_vectors, q.end_vector) - q.first_vector, start = v0 - q.first_vector;   // vectors of the slab
+    const int per = 1 << a.per_group_log2;
+    const int first = (int)threadIdx.x >> a.per_group_log2, part = (int)threadIdx.x & (per - 1), step = (int)blockDim.x >> a.per_group_log2;
     for (int pass = 0; pass < passes; pass++) {
         if (q.ty < a.rows) {
             double t[4] = {0, 0, 0, 0};
@@ -349,12 +375,15 @@ __device__ __forceinline__ void forward_group_sums(const GnArgs& a, const Place&
             const int at = base + first;
             double t1 = 0, t2 = 0;
             if (at < q.groups) {
-                const int c0 = (q.first_group + at) * a.group_channels;
-                const int lo = max(c0 / VEC, v0), hi = min((c0 + a.group_channels - 1) / VEC + 1, end);
+                const int c0 = at * a.group_channels;
+                const int lo = max(c0 / VEC, start), hi = min((c0 + a.group_channels - 1) / VEC + 1, end);
                 for (int w = lo; w < hi; w++) {
-                    const int slot = q.first_group + at - w * VEC / a.group_channels - 2 * pass;
+                    // which of its vector's groups this one is
+                    int slot = w * VEC < c0 ? 1 : 0;
+                    if (passes > 1) slot = at - group_of(a, w * VEC) - 2 * pass;
                     if (slot == 0 || slot == 1) {
-                        const double* from = lds + (w - v0) * 4 + slot * 2;
+                        const double* from = lds + (w - start) * 4 + slot * 2;
+                        #pragma unroll 2
                         for (int row = part; row < a.rows; row += per) {
                             t1 += from[row * a.slice_vectors * 4];
                             t2 += from[row * a.slice_vectors * 4 + 1];
@@ -362,8 +391,8 @@ __device__ __forceinline__ void forward_group_sums(const GnArgs& a, const Place&
                     }
                 }
             }
-            t1 = add_over(t1, per);
-            t2 = add_over(t2, per);
+            t1 = add_over(t1, a.per_group_log2);
+            t2 = add_over(t2, a.per_group_log2);
             if (at < q.groups && part == 0) {
                 sums[at][0] += t1;
                 sums[at][1] += t2;
@@ -378,7 +407,7 @@ __device__ __forceinline__ void write_stats(float* to, double mean, double squar
     double var = square - mean * mean;
     if (var < 0) var = 0;                                         // rounding; a NaN stays one
     to[0] = (float)mean;
-    to[1] = (float)(1.0 / sqrt(var + (double)eps));
+    to[1] = 1.0f / sqrtf((float)(var + (double)eps));             // three roundings of half a step
 }
 
 __device__ __forceinline__ void forward_stats(const GnArgs& a, const Place& q, long long n, double (*sums)[2], float (*stat)[2], bool write) {
@@ -403,7 +432,7 @@ __device__ __forceinline__ void load_stats(const float* from, const GnArgs& a, c
     __syncthreads();
 }
 
-template<typename T, int VEC, bool SILU, int B>
+template<typename T, int VEC, bool SILU, bool STREAM, int B>
 __device__ __forceinline__ void forward_apply(const GnArgs& a, const Lane<T, VEC>& lane, Vec<T, VEC> (&cur)[B], const float (&mean)[VEC],
                                               const float (&scale)[VEC], const float (&shift)[VEC]) {
     typedef Vec<T, VEC> V;
@@ -420,42 +449,42 @@ __device__ __forceinline__ void forward_apply(const GnArgs& a, const Lane<T, VEC
         return o;
     };
     int i = 0;
+    #pragma unroll 1
     for (; i + 2 * B <= lane.whole; i += B) {
         #pragma unroll
         for (int u = 0; u < B; u++) {
-            lane.store(a.out, i + u, one(cur[u]));
+            lane.template store<STREAM>(a.out, i + u, one(cur[u]));
             cur[u] = lane.load(a.x, i + B + u);
             in_order();
         }
     }
-    #pragma unroll
-    for (int u = 0; u < B; u++) {
-        if (i + u < lane.count) lane.store(a.out, i + u, one(cur[u]));
-        if (i + B + u < lane.runs) {
-            cur[u] = lane.load(a.x, i + B + u);
+    #pragma unroll 1
+    for (; i < lane.runs; i += B) {
+        #pragma unroll
+        for (int u = 0; u < B; u++) {
+            if (i + u < lane.count) lane.template store<STREAM>(a.out, i + u, one(cur[u]));
+            if (i + B + u < lane.runs) {
+                cur[u] = lane.load(a.x, i + B + u);
+            }
         }
-        in_order();
-    }
-    i += B;
-    if (i >= lane.runs) return;
-    #pragma unroll
-    for (int u = 0; u < B; u++) {
-        if (i + u < lane.count) lane.store(a.out, i + u, one(cur[u]));
     }
 }
 
 
-template<typename T, int VEC, int MODE>
+// ONE: a workgroup has one sample and its slab is one slice, as nearly always; the loops over them then go, and with
+// them the registers that what they repeat would hold.
+template<typename T, int VEC, int MODE, bool ONE>
 __global__ __launch_bounds__(kGroupNormMaxThreads, MODE == kBoth ? 2 : 4) void group_norm_forward(GnArgs a) {
     extern __shared__ double lds[];
     __shared__ double sums[kGroupNormMaxSlabGroups][2];
     __shared__ float stat[kGroupNormMaxSlabGroups][2];
-    const Place q = place_of(a, blockIdx.x);
-    for (long long n = q.n; n < a.batch; n += a.batch_blocks) {   // once, unless samples are shared out
+    const Place q = place_of(a, (int)blockIdx.x);
+    long long n = q.n;
+    do {
         constexpr int B = forward_batch(MODE);
-        Vec<T, VEC> pre[B];                                  // the first pixels of a slice
+        Vec<T, VEC> pre[B];                                       // the first pixels of a slice
         // whether they are the first slice's when the values are applied
-        const bool kept = MODE == kApply || q.end_vector - q.first_vector <= a.slice_vectors;
+        const bool kept = ONE || applies_only(MODE) || q.end_vector - q.first_vector <= a.slice_vectors;
         float scale[VEC], shift[VEC];
         {
             // on their way before anything else is done
@@ -468,14 +497,15 @@ __global__ __launch_bounds__(kGroupNormMaxThreads, MODE == kBoth ? 2 : 4) void g
                 }
             }
         }
-        if constexpr (MODE != kApply) {
+        if constexpr (!applies_only(MODE)) {
             clear_sums(q, sums);
-            for (int v0 = q.first_vector; v0 < q.end_vector; v0 += a.slice_vectors) {
+            int v0 = q.first_vector;
+            do {
                 const Lane<T, VEC> lane(a, q, n, v0);
                 float pivot[VEC], s1[VEC], s2[VEC];
                 int g[VEC];
                 if (lane.count) {
-                    if (v0 != q.first_vector) lane.load(pre, a.x, 0);
+                    if (!ONE && v0 != q.first_vector) lane.load(pre, a.x, 0);
                     groups_of<VEC>(g, a, q, lane.v);
                     if constexpr (MODE == kBoth) {
                         Vec<T, VEC> cur[B];                       // `pre` stays, to be applied
@@ -487,80 +517,87 @@ __global__ __launch_bounds__(kGroupNormMaxThreads, MODE == kBoth ? 2 : 4) void g
                     }
                 }
                 forward_group_sums<VEC>(a, q, v0, lane.count, g, pivot, s1, s2, lds, sums);
-            }
+                v0 += a.slice_vectors;
+            } while (!ONE && v0 < q.end_vector);
         }
         if constexpr (MODE == kSums) {
-            write_part(a, q, sums);
-            return;
-        }
-        if (MODE == kApply && a.finish) {
-            load_stats(a.stats, a, q, n, stat);
+            write_part(a, q, n, sums);
         } else {
-            if constexpr (MODE == kApply) gather_chunks(a, q, lds, sums);
-            forward_stats(a, q, n, sums, stat, q.chunk == 0);
-        }
-        for (int v0 = q.first_vector; v0 < q.end_vector; v0 += a.slice_vectors) {
-            const Lane<T, VEC> lane(a, q, n, v0);
-            if (!lane.count) continue;
-            if (!kept || v0 != q.first_vector) lane.load(pre, a.x, 0);
-            if (v0 != q.first_vector) {
-                load_params<T, VEC>(scale, a.weight, a.weight_fp32, lane.v * VEC, 1.0f);
-                load_params<T, VEC>(shift, a.bias, a.weight_fp32, lane.v * VEC, 0.0f);
+            if (applies_only(MODE) && a.finish) {
+                load_stats(a.stats, a, q, n, stat);
+            } else {
+                if constexpr (applies_only(MODE)) gather_chunks(a, q, n, lds, sums);
+                forward_stats(a, q, n, sums, stat, q.chunk == 0);
             }
-            float mean[VEC];
-            int g[VEC];
-            groups_of<VEC>(g, a, q, lane.v);
-            #pragma unroll
-            for (int j = 0; j < VEC; j++) {
-                mean[j] = stat[g[j]][0];
-                scale[j] *= stat[g[j]][1];
-            }
-            if (a.activation == kGroupNormSilu) forward_apply<T, VEC, true, B>(a, lane, pre, mean, scale, shift);
-            else forward_apply<T, VEC, false, B>(a, lane, pre, mean, scale, shift);
+            int v0 = q.first_vector;
+            do {
+                const Lane<T, VEC> lane(a, q, n, v0);
+                if (lane.count) {
+                    if (!kept || (!ONE && v0 != q.first_vector)) lane.load(pre, a.x, 0);
+                    if (!ONE && v0 != q.first_vector) {
+                        load_params<T, VEC>(scale, a.weight, a.weight_fp32, lane.v * VEC, 1.0f);
+                        load_params<T, VEC>(shift, a.bias, a.weight_fp32, lane.v * VEC, 0.0f);
+                    }
+                    float mean[VEC];
+                    int g[VEC];
+                    groups_of<VEC>(g, a, q, lane.v);
+                    #pragma unroll
+                    for (int j = 0; j < VEC; j++) {
+                        mean[j] = stat[g[j]][0];
+                        scale[j] *= stat[g[j]][1];
+                    }
+                    if (a.activation == kGroupNormSilu) forward_apply<T, VEC, true, MODE == kApplyStream, B>(a, lane, pre, mean, scale, shift);
+                    else forward_apply<T, VEC, false, MODE == kApplyStream, B>(a, lane, pre, mean, scale, shift);
+                }
+                v0 += a.slice_vectors;
+            } while (!ONE && v0 < q.end_vector);
         }
-        __syncthreads();
-    }
+        if constexpr (!ONE) __syncthreads();
+        n += gridDim.z;
+    } while (!ONE && n < a.batch);
 }
 
 // Adds up the chunks' sums of four groups of a sample and leaves what the last launch reads: forward the
 // statistics, backward the two means.
 template<bool BACKWARD>
 __global__ __launch_bounds__(256) void group_norm_finish(GnArgs a) {
-    __shared__ double lds[256 * 2];
-    const unsigned int quads = (unsigned int)(a.slab_groups + 3) / 4;
-    const unsigned int sample_slab = blockIdx.x / quads, quad = blockIdx.x - sample_slab * quads;
-    const unsigned int n = sample_slab / (unsigned int)a.slabs, slab = sample_slab - n * (unsigned int)a.slabs;
-    const int of = (int)threadIdx.x % 4, in_slab = (int)quad * 4 + of, g = (int)slab * a.slab_groups + in_slab;
+    __shared__ double2 lds[256];
+    const int in_slab = (int)(blockIdx.x * 4 + threadIdx.x % 4), g = (int)blockIdx.y * a.slab_groups + in_slab;
     const bool on = in_slab < a.slab_groups && g < a.groups;
-    double s1 = 0, s2 = 0;
-    if (on) {
-        const double* part = a.group_part + ((long long)sample_slab * a.chunks * a.slab_groups + in_slab) * 2;
-        #pragma unroll 4
-        for (int k = (int)threadIdx.x / 4; k < a.chunks; k += 64) {
-            const double* at = part + (long long)k * a.slab_groups * 2;
-            s1 += at[0];
-            s2 += at[1];
+    for (long long n = blockIdx.z; n < a.batch; n += gridDim.z) {
+        double2 t = {0, 0};
+        if (on) {
+            const double2* part = (const double2*)a.group_part + (n * gridDim.y + blockIdx.y) * a.chunks * a.slab_groups + in_slab;
+            for (int k = (int)threadIdx.x / 4; k < a.chunks; k += 8 * 64) {
+                double2 in[8];
+                #pragma unroll
+                for (int u = 0; u < 8; u++) in[u] = part[(long long)min(k + u * 64, a.chunks - 1) * a.slab_groups];
+                #pragma unroll
+                for (int u = 0; u < 8; u++) {
+                    t.x += k + u * 64 < a.chunks ? in[u].x : 0.0;
+                    t.y += k + u * 64 < a.chunks ? in[u].y : 0.0;
+                }
+            }
         }
-    }
-    lds[threadIdx.x * 2] = s1;
-    lds[threadIdx.x * 2 + 1] = s2;
-    for (int half = 128; half >= 4; half /= 2) {
+        lds[threadIdx.x] = t;
+        for (int half = 128; half >= 4; half /= 2) {
+            __syncthreads();
+            if ((int)threadIdx.x < half) {
+                lds[threadIdx.x].x += lds[threadIdx.x + half].x;
+                lds[threadIdx.x].y += lds[threadIdx.x + half].y;
+            }
+        }
+        if (threadIdx.x < 4 && on) {
+            t = lds[threadIdx.x];
+            float* to = (BACKWARD ? a.means : a.stats) + (n * a.groups + g) * 2;
+            if constexpr (BACKWARD) {
+                to[0] = (float)(t.x * a.inv_count);
+                to[1] = (float)(t.y * a.inv_count);
+            } else {
+                write_stats(to, t.x * a.inv_count, t.y * a.inv_count, a.eps);
+            }
+        }
         __syncthreads();
-        if ((int)threadIdx.x < half) {
-            lds[threadIdx.x * 2] += lds[(threadIdx.x + half) * 2];
-            lds[threadIdx.x * 2 + 1] += lds[(threadIdx.x + half) * 2 + 1];
-        }
-    }
-    if (threadIdx.x < 4 && on) {
-        s1 = lds[threadIdx.x * 2] * a.inv_count;
-        s2 = lds[threadIdx.x * 2 + 1] * a.inv_count;
-        float* to = (BACKWARD ? a.means : a.stats) + ((long long)n * a.groups + g) * 2;
-        if constexpr (BACKWARD) {
-            to[0] = (float)s1;
-            to[1] = (float)s2;
-        } else {
-            write_stats(to, s1, s2, a.eps);
-        }
     }
 }
 
@@ -620,6 +657,7 @@ __device__ __forceinline__ void backward_lane_sums(const GnArgs& a, const Place&
         }
     };
     int i = 0;
+    #pragma unroll 1
     for (; i + 2 * B <= lane.whole; i += B) {
         #pragma unroll
         for (int u = 0; u < B; u++) {
@@ -629,20 +667,15 @@ __device__ __forceinline__ void backward_lane_sums(const GnArgs& a, const Place&
             in_order();
         }
     }
-    #pragma unroll
-    for (int u = 0; u < B; u++) {
-        if (i + u < lane.count) add(x[u], g[u]);
-        if (i + B + u < lane.runs) {
-            x[u] = lane.load(a.x, i + B + u);
-            g[u] = lane.load(a.dout, i + B + u);
-        }
-        in_order();
-    }
-    i += B;
-    if (i < lane.runs) {
+    #pragma unroll 1
+    for (; i < lane.runs; i += B) {
         #pragma unroll
         for (int u = 0; u < B; u++) {
             if (i + u < lane.count) add(x[u], g[u]);
+            if (i + B + u < lane.runs) {
+                x[u] = lane.load(a.x, i + B + u);
+                g[u] = lane.load(a.dout, i + B + u);
+            }
         }
     }
     #pragma unroll
@@ -655,43 +688,49 @@ template<typename T, int VEC>
 __device__ __forceinline__ void backward_group_sums(const GnArgs& a, const Place& q, int v0, bool on, const float (&s1)[VEC], const float (&s2)[VEC],
                                                     double* lds, double (*sums)[2], long long row, bool add_to_row) {
     const int slice_channels = a.slice_vectors * VEC;
-    const int c0 = v0 * VEC, c1 = min(v0 + a.slice_vectors, q.end_vector) * VEC;
-    float* lanes = (float*)lds;                                   // [row][channel of the slice]
-    double* totals = lds + (a.rows * slice_channels + 1) / 2;     // [which][channel]
+    const int c0 = v0 * VEC, here = min(v0 + a.slice_vectors, q.end_vector) * VEC - c0;      // channels of the slice
+    float* lanes = (float*)lds;                                   // [which][row][channel of the slice]
+    double* totals = lds + a.rows * slice_channels;               // [which][channel]
     float* to = a.channel_part + row * 2 * a.channels + c0;
-    #pragma unroll
-    for (int which = 0; which < 2; which++) {
-        if (q.ty < a.rows) {
-            float* at = lanes + q.ty * slice_channels + q.tx * VEC;
-            #pragma unroll
-            for (int j = 0; j < VEC; j++) at[j] = !on ? 0.0f : which ? s2[j] : s1[j];
+    if (q.ty < a.rows) {
+        float* at = lanes + q.ty * slice_channels + q.tx * VEC;
+        #pragma unroll
+        for (int j = 0; j < VEC; j++) {
+            at[j] = on ? s1[j] : 0.0f;
+            at[a.rows * slice_channels + j] = on ? s2[j] : 0.0f;
         }
-        __syncthreads();
-        for (int c = (int)threadIdx.x; c < c1 - c0; c += (int)blockDim.x) {
-            double t = 0;
-            for (int r = 0; r < a.rows; r++) t += lanes[r * slice_channels + c];
-            float* part = to + which * a.channels + c;
-            *part = add_to_row ? *part + (float)t : (float)t;
-            float w[1];
-            load_params<T, 1>(w, a.weight, a.weight_fp32, c0 + c, 1.0f);
-            totals[which * slice_channels + c] = t * w[0];
-        }
-        __syncthreads();
     }
-    const int per = threads_per_group(q.groups);
-    const int first = (int)threadIdx.x / per, part = (int)threadIdx.x % per, step = (int)blockDim.x / per;
+    __syncthreads();
+    for (int c = (int)threadIdx.x; c < here; c += (int)blockDim.x) {
+        float w[1];
+        load_params<T, 1>(w, a.weight, a.weight_fp32, c0 + c, 1.0f);
+        double t1 = 0, t2 = 0;
+        #pragma unroll 4
+        for (int r = 0; r < a.rows; r++) {
+            t1 += lanes[r * slice_channels + c];
+            t2 += lanes[(a.rows + r) * slice_channels + c];
+        }
+        to[c] = add_to_row ? to[c] + (float)t1 : (float)t1;
+        to[a.channels + c] = add_to_row ? to[a.channels + c] + (float)t2 : (float)t2;
+        totals[c] = t1 * w[0];
+        totals[slice_channels + c] = t2 * w[0];
+    }
+    __syncthreads();
+    const int per = 1 << a.per_group_log2, start = c0 - q.first_vector * VEC;                // channels of the slab
+    const int first = (int)threadIdx.x >> a.per_group_log2, part = (int)threadIdx.x & (per - 1), step = (int)blockDim.x >> a.per_group_log2;
     for (int base = 0; base < q.groups; base += step) {
         const int at = base + first;
-        const int lo = max((q.first_group + at) * a.group_channels, c0), hi = min((q.first_group + at + 1) * a.group_channels, c1);
+        const int lo = max(at * a.group_channels, start), hi = min((at + 1) * a.group_channels, start + here);
         double t1 = 0, t2 = 0;
         if (at < q.groups) {
+            #pragma unroll 2
             for (int c = lo + part; c < hi; c += per) {
-                t1 += totals[c - c0];
-                t2 += totals[slice_channels + c - c0];
+                t1 += totals[c - start];
+                t2 += totals[slice_channels + c - start];
             }
         }
-        t1 = add_over(t1, per);
-        t2 = add_over(t2, per);
+        t1 = add_over(t1, a.per_group_log2);
+        t2 = add_over(t2, a.per_group_log2);
         if (at < q.groups && part == 0) {
             sums[at][0] += t1;
             sums[at][1] += t2;
@@ -701,7 +740,7 @@ __device__ __forceinline__ void backward_group_sums(const GnArgs& a, const Place
 }
 
 // dx = rstd (w dz - c1 - h c2) as dz scale - (x - mean) e - d
-template<typename T, int VEC, bool SILU, int B>
+template<typename T, int VEC, bool SILU, bool STREAM, int B>
 __device__ __forceinline__ void backward_apply(const GnArgs& a, const Place& q, long long n, const Lane<T, VEC>& lane,
                                                Vec<T, VEC> (&x)[B], Vec<T, VEC> (&g)[B], float (*stat)[2]) {
     typedef Vec<T, VEC> V;
@@ -730,73 +769,85 @@ __device__ __forceinline__ void backward_apply(const GnArgs& a, const Place& q, 
         return o;
     };
     int i = 0;
+    #pragma unroll 1
     for (; i + 2 * B <= lane.whole; i += B) {
         #pragma unroll
         for (int u = 0; u < B; u++) {
-            lane.store(a.out, i + u, one(x[u], g[u]));
+            lane.template store<STREAM>(a.out, i + u, one(x[u], g[u]));
             x[u] = lane.load(a.x, i + B + u);
             g[u] = lane.load(a.dout, i + B + u);
             in_order();
         }
     }
-    #pragma unroll
-    for (int u = 0; u < B; u++) {
-        if (i + u < lane.count) lane.store(a.out, i + u, one(x[u], g[u]));
-        if (i + B + u < lane.runs) {
-            x[u] = lane.load(a.x, i + B + u);
-            g[u] = lane.load(a.dout, i + B + u);
+    #pragma unroll 1
+    for (; i < lane.runs; i += B) {
+        #pragma unroll
+        for (int u = 0; u < B; u++) {
+            if (i + u < lane.count) lane.template store<STREAM>(a.out, i + u, one(x[u], g[u]));
+            if (i + B + u < lane.runs) {
+                x[u] = lane.load(a.x, i + B + u);
+                g[u] = lane.load(a.dout, i + B + u);
+            }
         }
-        in_order();
-    }
-    i += B;
-    if (i >= lane.runs) return;
-    #pragma unroll
-    for (int u = 0; u < B; u++) {
-        if (i + u < lane.count) lane.store(a.out, i + u, one(x[u], g[u]));
     }
 }
 
-// dw and db: the channels' sums added over the rows of the workspace, 64 channels to a workgroup.
+// dw and db: the channels' sums added over the rows of the workspace, 16 channels to a workgroup.
 template<typename T>
-__device__ __forceinline__ void add_params(const GnArgs& a, long long block, double* lds) {
+__device__ __forceinline__ void add_params(const GnArgs& a, int block, double* lds) {
     constexpr int W = kGroupNormParamChannels;
     const int tx = (int)threadIdx.x % W, ty = (int)threadIdx.x / W, rows = (int)blockDim.x / W;
-    const int c = (int)block * W + tx;
-    double s1 = 0, s2 = 0;
+    const int c = block * W + tx;
+    double2* lanes = (double2*)lds;
+    double2 t = {0, 0};
     if (c < a.channels) {
-        for (long long r = ty; r < a.channel_rows; r += rows) {
-            s1 += a.channel_part[r * 2 * a.channels + c];
-            s2 += a.channel_part[r * 2 * a.channels + a.channels + c];
+        const float* part = a.channel_part + c;
+        for (long long r = ty; r < a.channel_rows; r += 8 * rows) {
+            float in[8], in2[8];                                  // eight at a time, so that they are waited for once
+            #pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const float* at = part + min(r + u * rows, a.channel_rows - 1) * 2 * a.channels;
+                in[u] = at[0];
+                in2[u] = at[a.channels];
+            }
+            #pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const bool on = r + u * rows < a.channel_rows;
+                t.x += on ? in[u] : 0.0f;
+                t.y += on ? in2[u] : 0.0f;
+            }
         }
     }
-    lds[threadIdx.x * 2] = s1;
-    lds[threadIdx.x * 2 + 1] = s2;
+    lanes[threadIdx.x] = t;
     __syncthreads();
     if (ty == 0 && c < a.channels) {
+        #pragma unroll 4
         for (int i = 1; i < rows; i++) {
-            s1 += lds[(i * W + tx) * 2];
-            s2 += lds[(i * W + tx) * 2 + 1];
+            t.x += lanes[i * W + tx].x;
+            t.y += lanes[i * W + tx].y;
         }
-        store_param<T>(a.dbias, a.weight_fp32, c, (float)s1);
-        store_param<T>(a.dweight, a.weight_fp32, c, (float)s2);
+        store_param<T>(a.dbias, a.weight_fp32, c, (float)t.x);
+        store_param<T>(a.dweight, a.weight_fp32, c, (float)t.y);
     }
 }
 
-template<typename T, int VEC, int MODE>
+template<typename T, int VEC, int MODE, bool ONE>
 __global__ __launch_bounds__(kGroupNormMaxThreads, MODE == kBoth ? 2 : 4) void group_norm_backward(GnArgs a) {
     extern __shared__ double lds[];
     __shared__ double sums[kGroupNormMaxSlabGroups][2];
     __shared__ float stat[kGroupNormMaxSlabGroups][2];
-    if (MODE == kApply && blockIdx.x >= a.main_blocks) {
-        add_params<T>(a, blockIdx.x - a.main_blocks, lds);
+    if (applies_only(MODE) && (int)blockIdx.x < a.param_x) {          // a part of the grid that comes first
+        const long long block = ((long long)blockIdx.z * gridDim.y + blockIdx.y) * a.param_x + blockIdx.x;
+        if (block < a.param_blocks) add_params<T>(a, (int)block, lds);
         return;
     }
-    const Place q = place_of(a, blockIdx.x);
+    const Place q = place_of(a, (int)blockIdx.x - (applies_only(MODE) ? a.param_x : 0));
     const bool silu = a.activation == kGroupNormSilu;
-    for (long long n = q.n; n < a.batch; n += a.batch_blocks) {
+    long long n = q.n;
+    do {
         constexpr int B = backward_batch(MODE);
         Vec<T, VEC> px[B], pg[B];
-        const bool kept = MODE == kApply || q.end_vector - q.first_vector <= a.slice_vectors;
+        const bool kept = ONE || applies_only(MODE) || q.end_vector - q.first_vector <= a.slice_vectors;
         {
             const Lane<T, VEC> lane(a, q, n, q.first_vector);
             if (lane.count) {
@@ -804,13 +855,14 @@ __global__ __launch_bounds__(kGroupNormMaxThreads, MODE == kBoth ? 2 : 4) void g
                 lane.load(pg, a.dout, 0);
             }
         }
-        if constexpr (MODE != kApply) {
+        if constexpr (!applies_only(MODE)) {
             clear_sums(q, sums);
-            for (int v0 = q.first_vector; v0 < q.end_vector; v0 += a.slice_vectors) {
+            int v0 = q.first_vector;
+            do {
                 const Lane<T, VEC> lane(a, q, n, v0);
                 float s1[VEC], s2[VEC];
                 if (lane.count) {
-                    if (v0 != q.first_vector) {
+                    if (!ONE && v0 != q.first_vector) {
                         lane.load(px, a.x, 0);
                         lane.load(pg, a.dout, 0);
                     }
@@ -828,34 +880,39 @@ __global__ __launch_bounds__(kGroupNormMaxThreads, MODE == kBoth ? 2 : 4) void g
                     }
                 }
                 backward_group_sums<T, VEC>(a, q, v0, lane.count != 0, s1, s2, lds, sums, q.n * a.chunks + q.chunk, n != q.n);
-            }
+                v0 += a.slice_vectors;
+            } while (!ONE && v0 < q.end_vector);
         }
         if constexpr (MODE == kSums) {
-            write_part(a, q, sums);
-            return;
-        }
-        if (MODE == kApply && a.finish) {
-            load_stats(a.means, a, q, n, stat);
+            write_part(a, q, n, sums);
         } else {
-            if constexpr (MODE == kApply) gather_chunks(a, q, lds, sums);
-            for (int g = (int)threadIdx.x; g < q.groups; g += (int)blockDim.x) {
-                stat[g][0] = (float)(sums[g][0] * a.inv_count);
-                stat[g][1] = (float)(sums[g][1] * a.inv_count);
+            if (applies_only(MODE) && a.finish) {
+                load_stats(a.means, a, q, n, stat);
+            } else {
+                if constexpr (applies_only(MODE)) gather_chunks(a, q, n, lds, sums);
+                for (int g = (int)threadIdx.x; g < q.groups; g += (int)blockDim.x) {
+                    stat[g][0] = (float)(sums[g][0] * a.inv_count);
+                    stat[g][1] = (float)(sums[g][1] * a.inv_count);
+                }
+                __syncthreads();
             }
-            __syncthreads();
+            int v0 = q.first_vector;
+            do {
+                const Lane<T, VEC> lane(a, q, n, v0);
+                if (lane.count) {
+                    if (!kept || (!ONE && v0 != q.first_vector)) {
+                        lane.load(px, a.x, 0);
+                        lane.load(pg, a.dout, 0);
+                    }
+                    if (silu) backward_apply<T, VEC, true, MODE == kApplyStream, B>(a, q, n, lane, px, pg, stat);
+                    else backward_apply<T, VEC, false, MODE == kApplyStream, B>(a, q, n, lane, px, pg, stat);
+                }
+                v0 += a.slice_vectors;
+            } while (!ONE && v0 < q.end_vector);
         }
-        for (int v0 = q.first_vector; v0 < q.end_vector; v0 += a.slice_vectors) {
-            const Lane<T, VEC> lane(a, q, n, v0);
-            if (!lane.count) continue;
-            if (!kept || v0 != q.first_vector) {
-                lane.load(px, a.x, 0);
-                lane.load(pg, a.dout, 0);
-            }
-            if (silu) backward_apply<T, VEC, true, B>(a, q, n, lane, px, pg, stat);
-            else backward_apply<T, VEC, false, B>(a, q, n, lane, px, pg, stat);
-        }
-        __syncthreads();
-    }
+        if constexpr (!ONE) __syncthreads();
+        n += gridDim.z;
+    } while (!ONE && n < a.batch);
 }
 
 template<typename T>
@@ -874,65 +931,91 @@ GnArgs args_of(const GroupNormCall& c) {
     a.group_part = (double*)c.workspace;
     a.means = (float*)((char*)c.workspace + p.group_part_bytes);
     a.channel_part = (float*)((char*)c.workspace + p.group_part_bytes + p.means_bytes);
-    a.batch = c.batch; a.pixels = c.pixels; a.batch_blocks = p.batch_blocks;
-    a.channel_rows = p.channel_rows; a.main_blocks = p.blocks;
+    a.batch = c.batch; a.pixels = c.pixels; a.channel_rows = p.channel_rows;
     a.inv_count = 1.0 / ((double)c.pixels * (double)p.group_channels);
+    a.inv_group_channels = 1.0f / (float)p.group_channels; a.eps = c.eps;
+    a.gather_groups = p.slab_groups < p.threads ? p.slab_groups : p.threads;
+    a.gather_threads = p.threads / a.gather_groups;
+    a.inv_slice = ((1u << 20) + p.slice_vectors - 1) / p.slice_vectors;
+    a.inv_gather = ((1u << 20) + a.gather_groups - 1) / a.gather_groups;
     a.channels = c.channels; a.groups = c.groups; a.group_channels = p.group_channels; a.row_vectors = p.row_vectors;
-    a.slab_vectors = p.slab_vectors; a.slabs = p.slabs; a.slab_groups = p.slab_groups; a.slice_vectors = p.slice_vectors;
+    a.slab_vectors = p.slab_vectors; a.slab_groups = p.slab_groups; a.slice_vectors = p.slice_vectors;
     a.rows = p.rows; a.chunks = p.chunks;
-    a.weight_fp32 = c.weight_fp32; a.activation = c.activation; a.finish = p.finish; a.eps = c.eps;
+    const long long runs = gn_ceil(c.pixels, p.rows);
+    a.runs = (int)(runs / p.chunks);
+    a.more_runs = (int)(runs % p.chunks);
+    a.last_pixels = (int)(c.pixels % p.rows);
+    a.last_chunk = a.last_pixels ? (int)((runs - 1) % p.chunks) : -1;
+    while (a.per_group_log2 < 6 && (p.slab_groups << (a.per_group_log2 + 1)) <= p.threads) a.per_group_log2++;
+    a.weight_fp32 = c.weight_fp32; a.activation = c.activation; a.finish = p.finish;
     return a;
 }
 
-template<typename T, int VEC>
+dim3 grid_of(const GroupNormPlan& p) { return dim3((unsigned)p.chunks, (unsigned)p.slabs, (unsigned)p.batch_blocks); }
+dim3 finish_grid_of(const GroupNormPlan& p) { return dim3((unsigned)(p.slab_groups + 3) / 4, (unsigned)p.slabs, (unsigned)p.batch_blocks); }
+
+template<typename T, int VEC, bool ONE>
 hipError_t forward_of(const GroupNormCall& c, hipStream_t stream) {
     const GroupNormPlan& p = c.plan;
     const GnArgs a = args_of(c);
-    const dim3 grid((unsigned)p.blocks), block((unsigned)p.threads);
+    const dim3 grid = grid_of(p), block((unsigned)p.threads);
     if (p.chunks == 1) {
-        group_norm_forward<T, VEC, kBoth><<<grid, block, p.lds_bytes, stream>>>(a);
+        group_norm_forward<T, VEC, kBoth, ONE><<<grid, block, p.lds_bytes, stream>>>(a);
         return hipGetLastError();
     }
-    group_norm_forward<T, VEC, kSums><<<grid, block, p.lds_bytes, stream>>>(a);
+    group_norm_forward<T, VEC, kSums, ONE><<<grid, block, p.lds_bytes, stream>>>(a);
     hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
     if (p.finish) {
-        group_norm_finish<false><<<dim3((unsigned)(c.batch * p.slabs * ((p.slab_groups + 3) / 4))), dim3(256), 0, stream>>>(a);
+        group_norm_finish<false><<<finish_grid_of(p), dim3(256), 0, stream>>>(a);
         err = hipGetLastError();
         if (err != hipSuccess) return err;
     }
-    group_norm_forward<T, VEC, kApply><<<grid, block, p.lds_bytes, stream>>>(a);
+    if (p.stream) group_norm_forward<T, VEC, kApplyStream, ONE><<<grid, block, p.lds_bytes, stream>>>(a);
+    else group_norm_forward<T, VEC, kApply, ONE><<<grid, block, p.lds_bytes, stream>>>(a);
     return hipGetLastError();
 }
 
-template<typename T, int VEC>
+template<typename T, int VEC, bool ONE>
 hipError_t backward_of(const GroupNormCall& c, hipStream_t stream) {
     const GroupNormPlan& p = c.plan;
-    const GnArgs a = args_of(c);
-    const dim3 grid((unsigned)p.blocks), block((unsigned)p.threads);
+    GnArgs a = args_of(c);
+    dim3 grid = grid_of(p);
+    const dim3 block((unsigned)p.threads);
+    const bool params = c.dweight || c.dbias;
     if (p.chunks == 1) {
-        group_norm_backward<T, VEC, kBoth><<<grid, block, p.lds_bytes, stream>>>(a);
+        group_norm_backward<T, VEC, kBoth, ONE><<<grid, block, p.lds_bytes, stream>>>(a);
         const hipError_t err = hipGetLastError();
-        if (err != hipSuccess || (!c.dweight && !c.dbias)) return err;
+        if (err != hipSuccess || !params) return err;
         group_norm_params<T><<<dim3((unsigned)p.param_blocks), dim3(256), 0, stream>>>(a);
         return hipGetLastError();
     }
-    group_norm_backward<T, VEC, kSums><<<grid, block, p.lds_bytes, stream>>>(a);
+    group_norm_backward<T, VEC, kSums, ONE><<<grid, block, p.lds_bytes, stream>>>(a);
     hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
     if (p.finish) {
-        group_norm_finish<true><<<dim3((unsigned)(c.batch * p.slabs * ((p.slab_groups + 3) / 4))), dim3(256), 0, stream>>>(a);
+        group_norm_finish<true><<<finish_grid_of(p), dim3(256), 0, stream>>>(a);
         err = hipGetLastError();
         if (err != hipSuccess) return err;
     }
-    const dim3 both((unsigned)(p.blocks + (c.dweight || c.dbias ? p.param_blocks : 0)));
-    group_norm_backward<T, VEC, kApply><<<both, block, p.lds_bytes, stream>>>(a);
+    if (params) {
+        a.param_blocks = p.param_blocks;
+        a.param_x = (int)gn_ceil(p.param_blocks, (long long)p.slabs * p.batch_blocks);
+        grid.x += (unsigned)a.param_x;
+    }
+    if (p.stream) group_norm_backward<T, VEC, kApplyStream, ONE><<<grid, block, p.lds_bytes, stream>>>(a);
+    else group_norm_backward<T, VEC, kApply, ONE><<<grid, block, p.lds_bytes, stream>>>(a);
     return hipGetLastError();
 }
 
 template<typename T, int VEC>
 hipError_t launch_of(const GroupNormCall& c, bool backward, hipStream_t stream) {
-    return backward ? backward_of<T, VEC>(c, stream) : forward_of<T, VEC>(c, stream);
+    // (instantiated for full vectors only: the others are built once, with the loops)
+    if constexpr (sizeof(T) * VEC == 16) {
+        if (c.plan.batch_blocks == c.batch && c.plan.slab_vectors <= c.plan.slice_vectors)
+            return backward ? backward_of<T, VEC, true>(c, stream) : forward_of<T, VEC, true>(c, stream);
+    }
+    return backward ? backward_of<T, VEC, false>(c, stream) : forward_of<T, VEC, false>(c, stream);
 }
 
 template<typename T>

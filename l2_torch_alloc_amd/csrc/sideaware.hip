@@ -106,6 +106,7 @@ struct Tuning {
 // launch on any thread, hence atomics.  Kernels carry the generation they were compiled under;
 // a change of a compiled-in knob bumps it and the next launch builds a fresh instantiation.
 constexpr int kTuneKnobs = 17;
+constexpr int kTuneCacheBytes = 3;                        // "cache_bytes"
 static const char* const kTuneNames[kTuneKnobs] = {"stripe_bytes", "slot_run", "one_shot", "cache_bytes",
                                                    "nt_store", "groups_cap", "wg_threads", "stripes_per_xcd",
                                                    "write_through", "sided", "sided_min_bytes", "sided_stripe",
@@ -1231,7 +1232,7 @@ static DeviceContext* plan_group_norm_call(const char* what, long long batch, lo
     }
     DeviceContext* ctx = get_context(device);
     if (!ctx) return nullptr;
-    *plan = plan_group_norm(batch, pixels, channels, groups, element, backward, ctx->num_cus);
+    *plan = plan_group_norm(batch, pixels, channels, groups, element, backward, ctx->num_cus, g_tune[kTuneCacheBytes].load(std::memory_order_relaxed));
     if (!plan->ok) {
         set_error("%s: %lld samples of %lld pixels, %d channels in %d groups do not fit one launch", what, batch, pixels, channels, groups);
         return nullptr;

@@ -34,13 +34,31 @@ int main() {
         REQUIRE((pixels + (long long)p.chunks * p.rows - 1) / ((long long)p.chunks * p.rows) <= kGroupNormMaxLanePixels);
         REQUIRE((long long)p.rows * channels * element <= kGroupNormMaxRowsBytes);
         // samples
-        const long long samples = p.chunks > 1 ? batch : p.batch_blocks;
-        REQUIRE(samples >= 1 && samples <= batch && p.blocks == samples * p.slabs * p.chunks);
-        REQUIRE(p.blocks + p.param_blocks <= 0x7fffffffll);
-        // LDS: forward four doubles a lane; backward a float for each lane's channel, rounded up to a double, and two
+        const long long samples = p.batch_blocks;
+        REQUIRE(samples >= 1 && samples <= batch && samples <= 65535 && p.slabs <= 65535 && p.blocks == samples * p.slabs * p.chunks);
+        const long long others = p.slabs * samples;
+        REQUIRE((p.chunks + (p.param_blocks + others - 1) / others) * others <= 0x7fffffffll);
+        // thread numbers are divided by multiplying with 2^20 / slice_vectors
+        for (int t = 0; t < p.threads; t++) {
+            const unsigned inv = ((1u << 20) + p.slice_vectors - 1) / p.slice_vectors;
+            REQUIRE((int)((t * inv) >> 20) == t / p.slice_vectors);
+            const int gather = p.slab_groups < p.threads ? p.slab_groups : p.threads;
+            const unsigned inv_gather = ((1u << 20) + gather - 1) / gather;
+            REQUIRE((int)((t * inv_gather) >> 20) == t / gather);
+        }
+        // ... and channels of a slab by the fp32 reciprocal of a group's, one step of correction either way
+        for (int g = 0; g <= p.slab_groups; g++) {
+            for (int d = -1; d <= 1; d++) {
+                const long long c = (long long)g * p.group_channels + d;
+                if (c < 0 || c >= (long long)p.slab_vectors * p.vec) continue;
+                const int guess = (int)((float)(int)c * (1.0f / (float)p.group_channels));
+                REQUIRE(guess - (int)(c / p.group_channels) <= 1 && (int)(c / p.group_channels) - guess <= 1);
+            }
+        }
+        // LDS: forward four doubles a lane; backward two floats for each lane's channel, and two
         // doubles for each channel of the slice; two doubles a thread
         const size_t slice_channels = (size_t)p.slice_vectors * p.vec;
-        if (backward) REQUIRE(p.lds_bytes >= (p.rows * slice_channels + 1) / 2 * 8 + 2 * slice_channels * 8);
+        if (backward) REQUIRE(p.lds_bytes >= p.rows * slice_channels * 8 + 2 * slice_channels * 8);
         else REQUIRE(p.lds_bytes >= (size_t)p.slice_vectors * p.rows * 32);
         REQUIRE(p.lds_bytes >= (size_t)p.threads * 16);
         REQUIRE(p.lds_bytes + kGroupNormMaxSlabGroups * 24 <= 65536);
