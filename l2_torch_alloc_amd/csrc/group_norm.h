@@ -52,6 +52,7 @@ constexpr int kGroupNormMaxSlabGroups = 256;
 constexpr int kGroupNormParamChannels = 16;       // channels per workgroup that adds up their sums
 constexpr long long kGroupNormMaxLanePixels = 256;
 constexpr long long kGroupNormOneLaunchBytes = 32 << 10;
+constexpr long long kGroupNormPiecesBytes = 8 << 20;
 constexpr long long kGroupNormGatherBytes = 64 << 10;
 constexpr long long kGroupNormMaxGrid = 65535;            // of the second and third axis
 constexpr long long kGroupNormMaxRowsBytes = 1ll << 30;    // a lane's offset among the rows has 32 bits
@@ -94,12 +95,14 @@ inline GroupNormPlan plan_group_norm(long long batch, long long pixels, int chan
     // time out of its caches.  Else the pixels are cut into chunks as well, and a second launch applies
     // what the first one summed.
     const long long unit_bytes = pixels * unit_vectors * p.vec * element_bytes;
-    if (unit_bytes <= kGroupNormOneLaunchBytes) {
-        int m = 1;
-        // wider slabs while there are workgroups enough without, up to 512 bytes of a row
-        while (2 * m <= most_units && 2 * m * unit_vectors <= 32 && batch * gn_ceil(units, 2 * m) >= 2 * num_cus &&
-               2 * m * unit_bytes <= kGroupNormOneLaunchBytes)
-            m *= 2;
+    // wider slabs while there are workgroups enough without, up to 512 bytes of a row
+    int m = 1;
+    while (2 * m <= most_units && 2 * m * unit_vectors <= 32 && batch * gn_ceil(units, 2 * m) >= 2 * num_cus &&
+           2 * m * unit_bytes <= kGroupNormOneLaunchBytes)
+        m *= 2;
+    // (pieces of less than a memory line are all right for little, not for much)
+    const bool pieces = m * unit_vectors * p.vec * element_bytes < 128 && m < units;
+    if (unit_bytes <= kGroupNormOneLaunchBytes && !(pieces && batch * pixels * row_bytes > kGroupNormPiecesBytes)) {
         cut(m);
         const long long want = gn_ceil(4ll * num_cus, p.slabs);
         p.batch_blocks = batch < want ? batch : want;

@@ -474,7 +474,7 @@ __device__ __forceinline__ void forward_apply(const GnArgs& a, const Lane<T, VEC
 // ONE: a workgroup has one sample and its slab is one slice, as nearly always; the loops over them then go, and with
 // them the registers that what they repeat would hold.
 template<typename T, int VEC, int MODE, bool ONE>
-__global__ __launch_bounds__(kGroupNormMaxThreads, MODE == kBoth ? 2 : 4) void group_norm_forward(GnArgs a) {
+__global__ __launch_bounds__(kGroupNormMaxThreads, 4) void group_norm_forward(GnArgs a) {
     extern __shared__ double lds[];
     __shared__ double sums[kGroupNormMaxSlabGroups][2];
     __shared__ float stat[kGroupNormMaxSlabGroups][2];
@@ -603,7 +603,7 @@ __global__ __launch_bounds__(256) void group_norm_finish(GnArgs a) {
 
 // ---- backward ----------------------------------------------------------------------------------
 
-constexpr int backward_batch(int mode) { return mode == kBoth ? 3 : 2; }      // pixels of both arrays
+constexpr int backward_batch(int) { return 2; }                               // pixels of both arrays
 
 // dz of a value from z
 template<bool SILU>
@@ -832,7 +832,7 @@ __device__ __forceinline__ void add_params(const GnArgs& a, int block, double* l
 }
 
 template<typename T, int VEC, int MODE, bool ONE>
-__global__ __launch_bounds__(kGroupNormMaxThreads, MODE == kBoth ? 2 : 4) void group_norm_backward(GnArgs a) {
+__global__ __launch_bounds__(kGroupNormMaxThreads, 4) void group_norm_backward(GnArgs a) {
     extern __shared__ double lds[];
     __shared__ double sums[kGroupNormMaxSlabGroups][2];
     __shared__ float stat[kGroupNormMaxSlabGroups][2];
