@@ -8,9 +8,9 @@ even and sin at odd columns.
 """
 from __future__ import annotations
 
-import ctypes
 import math
 import os
+import struct
 from typing import Dict, Optional, Tuple
 
 import torch
@@ -147,28 +147,26 @@ def rope_backward_heads(dout, freqs, out=None, positions=None):
     return _rope(dout, freqs, out, 0, 0, "heads", True, positions)
 
 
-class _Segment(ctypes.Structure):
-    """``sideaware_segment`` of include/sideaware.h."""
-    _fields_ = [("num_bytes", ctypes.c_size_t), ("out", ctypes.c_void_p * 4), ("inp", ctypes.c_void_p * 4),
-                ("sideband_memory", ctypes.c_void_p), ("sideband_value", ctypes.c_int)]
+# ``sideaware_segment`` of include/sideaware.h: num_bytes, out[4], in[4], sideband_memory, sideband_value
+_SEGMENT = struct.Struct("=Q4Q4QQi4x")
 
 
 def elementwise_batch(kernel_id: int, segments) -> None:
     """One launch over several arrays of the same op.  ``segments`` is a sequence of
     ``(num_bytes, outs, ins, sideband_tensor_or_None, sideband_value)`` with ``outs`` / ``ins``
     sequences of up to four tensors (or None)."""
-    arr = (_Segment * len(segments))()
-    first = next((t for seg in segments for t in list(seg[1]) + list(seg[2]) if t is not None), None)
-    for seg, (num_bytes, outs, ins, sideband, value) in zip(arr, segments):
-        seg.num_bytes = num_bytes
+    packed, first = [], None
+    for num_bytes, outs, ins, sideband, value in segments:
+        out, inp = [0] * 4, [0] * 4
         for i, t in enumerate(outs):
-            seg.out[i] = wrapper._check(t, "out%d" % i) or None
+            out[i] = wrapper._check(t, "out%d" % i)
+            first = t if first is None else first
         for i, t in enumerate(ins):
-            seg.inp[i] = wrapper._check(t, "in%d" % i) or None
-        seg.sideband_memory = sideband.data_ptr() if sideband is not None else None
-        seg.sideband_value = int(value)
+            inp[i] = wrapper._check(t, "in%d" % i)
+            first = t if first is None else first
+        packed.append(_SEGMENT.pack(num_bytes, *out, *inp, sideband.data_ptr() if sideband is not None else 0, int(value)))
     device, stream = wrapper._device_and_stream(first)      # where the arrays live, the current device or not
-    wrapper.library().sideaware_elementwise_batch(kernel_id, len(arr), arr, device, stream)
+    wrapper.library().sideaware_elementwise_batch(kernel_id, len(packed), b"".join(packed), device, stream)
 
 
 def _rope_heads_many(tensors, freqs: torch.Tensor, backward: bool, positions: Optional[torch.Tensor] = None):
@@ -291,33 +289,73 @@ def freqs_cis_axes_table(sections, end: int, theta: float, order: str = "blocks"
     return torch.stack([angle.cos(), angle.sin()], -1).reshape(end, 2 * len(axis)).float()
 
 
+# What calls of the ops below need besides their pointers, by everything it depends on (shapes, types, devices and
+# options, never a tensor): the checks of those are made once for each.
+_PLANS_KEPT = 4096
+_plans: Dict[Tuple, Tuple] = {}
+
+
+def _keep_plan(key: Tuple, plan: Tuple) -> Tuple:
+    if len(_plans) >= _PLANS_KEPT:
+        _plans.clear()
+    _plans[key] = plan
+    return plan
+
+
+def _aligned(t: torch.Tensor, name: str) -> int:
+    """Address of a tensor whose device is known: contiguous and 16-byte aligned."""
+    assert t.is_contiguous(), name + " must be contiguous"
+    ptr = t.data_ptr()
+    assert not ptr & 15, name + " must be 16-byte aligned"
+    return ptr
+
+
+def _rope_axes_plan(shapes, out_shapes, dtypes, devices, freqs_shape, positions_shape, sections, half, order, backward):
+    """The kernel and, for each tensor with elements, its bytes and sideband value."""
+    first = shapes[0]
+    assert len(first) == 4, "activations are (B, T, heads, head_dim)"
+    B, T, _, head_dim = first
+    dtype = _ROPE_DTYPES.get(dtypes[0])
+    if dtype is None:
+        raise TypeError("RoPE storage is float32, bfloat16 or float16")
+    freqs_type, positions_type = dtypes[-2:]
+    assert freqs_type == torch.float32 and len(freqs_shape) == 2 and freqs_shape[1] == head_dim, "the table is float32, (rows, head_dim)"
+    assert positions_type == torch.int32, "positions are a contiguous int32 tensor"
+    assert tuple(positions_shape) in ((B, T, len(sections)), (B * T, len(sections))), \
+        "positions are (B, T, axes): one row of the table for each axis of every token"
+    assert len(out_shapes) == len(shapes), "one output per tensor"
+    for t, o in zip(shapes, out_shapes):
+        assert len(t) == 4 and t[:2] == first[:2] and t[3] == head_dim, "tensors share B, T and head_dim"
+        assert o == t, "an output is like its tensor"
+    assert all(d == dtypes[0] for d in dtypes[:-2]), "tensors and outputs share one type"
+    assert devices[0] >= 0 and all(d == devices[0] for d in devices), "tensors, outputs, table and positions live on one GPU"
+    kid = _kernel("rope_axes", (head_dim, sections, dtype, half, order, backward))
+    size = 4 if dtype == "fp32" else 2
+    return kid, [(t.numel() * size, headers.rope_axes_sideband(t[2], freqs_shape[0])) for t in shapes]
+
+
 def _rope_axes_many(tensors, freqs, positions, sections, half: bool, order: str, backward: bool, outs):
     tensors = list(tensors)
     outs = tensors if outs is None else list(outs)
-    first = tensors[0]
-    assert first.dim() == 4, "activations are (B, T, heads, head_dim)"
-    B, T, _, head_dim = first.shape
-    dtype = _ROPE_DTYPES.get(first.dtype)
-    if dtype is None:
-        raise TypeError("RoPE storage is float32, bfloat16 or float16")
-    sections = tuple(int(n) for n in sections)
-    assert freqs.dtype == torch.float32 and freqs.dim() == 2 and freqs.shape[1] == head_dim, \
-        "the table is float32, (rows, head_dim)"
-    assert positions.dtype == torch.int32 and positions.is_contiguous(), "positions are a contiguous int32 tensor"
-    assert tuple(positions.shape) in ((B, T, len(sections)), (B * T, len(sections))), \
-        "positions are (B, T, axes): one row of the table for each axis of every token"
-    assert len(outs) == len(tensors), "one output per tensor"
-    for t, o in zip(tensors, outs):
-        assert t.dim() == 4 and t.shape[:2] == first.shape[:2] and t.shape[3] == head_dim and t.dtype == first.dtype, \
-            "tensors share B, T, head_dim and dtype"
-        assert o.shape == t.shape and o.dtype == t.dtype, "an output is like its tensor"
-        assert t.device == o.device == first.device, "tensors and outputs live on one device"
-    assert positions.device == first.device and freqs.device == first.device, "table and positions live on the activations' device"
-    kid = _kernel("rope_axes", (head_dim, sections, dtype, bool(half), order, backward))
-    work = [(t, o) for t, o in zip(tensors, outs) if t.numel()]
-    if work:
-        elementwise_batch(kid, [(t.numel() * t.element_size(), [o], [t, freqs, freqs, freqs], positions,
-                                 headers.rope_axes_sideband(t.shape[2], freqs.shape[0])) for t, o in work])
+    every = tensors + outs + [freqs, positions]
+    shapes, dtypes, devices = [t.shape for t in every], [t.dtype for t in every], [t.get_device() for t in every]
+    n = len(tensors)
+    key = ("rope_axes", n, tuple(shapes), tuple(dtypes), tuple(devices), tuple(sections), bool(half), order, backward)
+    assert positions.is_contiguous(), "positions are a contiguous int32 tensor"
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _keep_plan(key, _rope_axes_plan(shapes[:n], shapes[n:-2], dtypes, devices, freqs.shape, positions.shape,
+                                               tuple(int(s) for s in sections), bool(half), order, backward))
+    kid, sizes = plan
+    if all(num_bytes for num_bytes, _ in sizes):
+        table, where = _aligned(freqs, "freqs"), positions.data_ptr()
+        packed = b"".join([_SEGMENT.pack(num_bytes, _aligned(o, "out"), 0, 0, 0, _aligned(t, "x"), table, table, table, where, value)
+                           for t, o, (num_bytes, value) in zip(tensors, outs, sizes)])
+        device, stream = wrapper._device_and_stream(freqs)
+        wrapper.library().sideaware_elementwise_batch(kid, n, packed, device, stream)
+    elif any(num_bytes for num_bytes, _ in sizes):             # tensors without heads among others
+        some = [i for i in range(n) if sizes[i][0]]
+        _rope_axes_many([tensors[i] for i in some], freqs, positions, sections, half, order, backward, [outs[i] for i in some])
     return outs
 
 
@@ -363,15 +401,23 @@ def _dropout(x: torch.Tensor, p: float, seed: torch.Tensor, residual: Optional[t
     dtype = _ROPE_DTYPES.get(x.dtype)
     if dtype is None:
         raise TypeError("dropout storage is float32, bfloat16 or float16")
-    assert seed.dtype == torch.int64 and seed.numel() == 2 and seed.is_contiguous() and seed.device == x.device, \
+    device = x.get_device()
+    assert seed.dtype == torch.int64 and seed.numel() == 2 and seed.is_contiguous() and seed.get_device() == device, \
         "the seed is an int64 tensor of two values (seed, offset) on the activations' device"
     if residual is not None:
-        assert residual.shape == x.shape and residual.dtype == x.dtype and residual.device == x.device, \
-            "the residual is like the activation"
+        assert residual.shape == x.shape and residual.dtype == x.dtype and residual.get_device() == device, "the residual is like the activation"
     out = _like(out, x, "out")
     if x.numel():
-        kid = _kernel("dropout", (dtype, residual is not None))
-        _elementwise(kid, out, None, None, None, x, residual, None, None, seed, threshold, 0, 0)
+        kid = _kernel_ids.get(("dropout", (dtype, residual is not None), ()))
+        if kid is None or torch.compiler.is_compiling():
+            kid = _kernel("dropout", (dtype, residual is not None))
+            _elementwise(kid, out, None, None, None, x, residual, None, None, seed, threshold, 0, 0)
+        else:
+            assert x.is_cuda, "x must be on the GPU"
+            device, stream = wrapper._device_and_stream(x)
+            wrapper.library().sideaware_elementwise(kid, x.numel() * x.element_size(), _aligned(out, "out"), 0, 0, 0, _aligned(x, "x"),
+                                                    0 if residual is None else _aligned(residual, "residual"), 0, 0, seed.data_ptr(), threshold,
+                                                    0, 0, device, stream)
     return out
 
 
@@ -394,27 +440,43 @@ _GROUP_NORM_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTIVATIONS = {"none": 0, "silu": 1}
 
 
-def _group_norm_shape(x: torch.Tensor, weight, bias, groups: int, activation: str):
-    """(batch, pixels, channels, type, weight_fp32, activation) of a call, checked."""
-    dtype = _GROUP_NORM_TYPES.get(x.dtype)
+def _group_norm_plan(shape, dtype_of_x, device, params, groups: int, activation: str):
+    """(batch, pixels, channels, type, weight_fp32, activation, bytes of workspace forward and backward) of a call, its
+    sizes, types and devices checked; ``params`` are the (shape, type, device) of weight and bias, or None."""
+    dtype = _GROUP_NORM_TYPES.get(dtype_of_x)
     if dtype is None:
         raise TypeError("group norm storage is float32, bfloat16 or float16")
     if activation not in _ACTIVATIONS:
         raise ValueError("the activation is 'none' or 'silu'")
-    assert x.dim() >= 2, "activations are (N, ..., C), channels last"
-    batch, channels = x.shape[0], x.shape[-1]
+    assert len(shape) >= 2, "activations are (N, ..., C), channels last"
+    batch, channels = shape[0], shape[-1]
     if groups < 1 or channels < 1 or channels % groups:
         raise ValueError("%d groups do not divide %d channels" % (groups, channels))
-    pixels = x[0].numel() // channels if batch else 1
+    pixels = 1
+    for n in shape[1:-1]:
+        pixels *= n
     if pixels < 1:
         raise ValueError("a sample without pixels has no mean")
-    params = [t for t in (weight, bias) if t is not None]
-    for t in params:
-        assert t.dtype in (torch.float32, x.dtype) and t.dtype == params[0].dtype, "weight and bias are both float32 or both of the activations' type"
-        assert tuple(t.shape) == (channels,) and t.is_contiguous() and t.device == x.device, \
-            "weight and bias have one value per channel, on the activations' device"
-    weight_fp32 = 1 if not params or params[0].dtype == torch.float32 else 0
-    return batch, pixels, channels, dtype, weight_fp32, _ACTIVATIONS[activation]
+    params = [t for t in params if t is not None]
+    for of_shape, of_type, of_device in params:
+        assert of_type in (torch.float32, dtype_of_x) and of_type == params[0][1], "weight and bias are both float32 or both of the activations' type"
+        assert tuple(of_shape) == (channels,) and of_device == device, "weight and bias have one value per channel, on the activations' device"
+    weight_fp32 = 1 if not params or params[0][1] == torch.float32 else 0
+    need = [0, 0]
+    if batch and device >= 0:
+        need = [wrapper.library().sideaware_group_norm_workspace(batch, pixels, channels, groups, dtype, backward, device) for backward in (0, 1)]
+    return batch, pixels, channels, dtype, weight_fp32, _ACTIVATIONS[activation], need
+
+
+def _group_norm_call(x: torch.Tensor, weight, bias, groups: int, activation: str):
+    device = x.get_device()
+    params = tuple(None if t is None else (t.shape, t.dtype, t.get_device()) for t in (weight, bias))
+    key = ("group_norm", x.shape, x.dtype, device, params, groups, activation)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _keep_plan(key, _group_norm_plan(x.shape, x.dtype, device, params, groups, activation))
+    assert (weight is None or weight.is_contiguous()) and (bias is None or bias.is_contiguous()), "weight and bias are contiguous"
+    return plan
 
 
 def _may_allocate(what: str) -> None:
@@ -428,32 +490,34 @@ def _like(t, x: torch.Tensor, name: str) -> torch.Tensor:
     if t is None:
         _may_allocate(name)
         return torch.empty_like(x)
-    assert t.shape == x.shape and t.dtype == x.dtype and t.device == x.device, name + " is like the activation"
+    assert t.shape == x.shape and t.dtype == x.dtype and t.get_device() == x.get_device(), name + " is like the activation"
     return t
 
 
-def _group_norm_workspace(workspace, batch, pixels, channels, groups, dtype, backward: bool, device: int):
-    need = wrapper.library().sideaware_group_norm_workspace(batch, pixels, channels, groups, dtype, int(backward), device)
+def _workspace(workspace, need: int, x: torch.Tensor):
+    """(address, bytes, tensor) of a call's workspace."""
     if workspace is None:
         if need == 0:
             return 0, 0, None
         _may_allocate("workspace")
-        workspace = torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", device))
-    assert workspace.is_cuda and workspace.get_device() == device and workspace.is_contiguous() and workspace.data_ptr() % 16 == 0, \
-        "the workspace is a contiguous tensor on the activations' device"
-    return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
+        workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+        return workspace.data_ptr(), need, workspace
+    assert workspace.get_device() == x.get_device(), "the workspace lives on the activations' device"
+    return _aligned(workspace, "workspace"), workspace.numel() * workspace.element_size(), workspace
 
 
 def group_norm_workspace(x: torch.Tensor, groups: int, backward: bool = False) -> int:
     """The bytes of ``workspace`` that :func:`group_norm_forward` (or backward) of ``x`` needs; may be 0."""
-    batch, pixels, channels, dtype, _, _ = _group_norm_shape(x, None, None, groups, "none")
-    if batch == 0:
-        return 0
-    return wrapper.library().sideaware_group_norm_workspace(batch, pixels, channels, groups, dtype, int(backward), x.get_device())
+    return _group_norm_call(x, None, None, groups, "none")[6][1 if backward else 0]
 
 
 def _group_norm_failed(what: str):
     raise RuntimeError("%s: %s" % (what, wrapper.sideaware_last_error()))
+
+
+def _check_stats(stats: torch.Tensor, batch: int, groups: int, x: torch.Tensor) -> None:
+    assert stats.shape == (batch, groups, 2) and stats.dtype == torch.float32 and stats.is_contiguous() and stats.get_device() == x.get_device(), \
+        "stats are float32 (N, groups, 2)"
 
 
 def group_norm_forward(x, weight, bias, groups: int, eps: float = 1e-5, activation: str = "none", out=None, stats=None, workspace=None):
@@ -466,21 +530,21 @@ def group_norm_forward(x, weight, bias, groups: int, eps: float = 1e-5, activati
     ``out`` (may be ``x``), ``stats`` and ``workspace`` (:func:`group_norm_workspace` bytes, of any type) are
     allocated unless given.  Under stream capture with this library's allocator they have to be given, and calls that can
     overlap, such as two graphs' replays, each need their own."""
-    batch, pixels, channels, dtype, weight_fp32, act = _group_norm_shape(x, weight, bias, groups, activation)
+    batch, pixels, channels, dtype, weight_fp32, act, need = _group_norm_call(x, weight, bias, groups, activation)
     out = _like(out, x, "out")
     if stats is None:
         _may_allocate("stats")
-        stats = torch.empty(batch, groups, 2, dtype=torch.float32, device=x.device)
-    assert tuple(stats.shape) == (batch, groups, 2) and stats.dtype == torch.float32 and stats.is_contiguous() and stats.device == x.device, \
-        "stats are float32 (N, groups, 2)"
+        stats = torch.empty((batch, groups, 2), dtype=torch.float32, device=x.device)
+    else:
+        _check_stats(stats, batch, groups, x)
     if batch == 0:
         return out, stats
-    x_ptr, out_ptr = wrapper._check(x, "x"), wrapper._check(out, "out")
+    assert x.is_cuda, "x must be on the GPU"
+    ws_ptr, ws_bytes, keep = _workspace(workspace, need[0], x)
     device, stream = wrapper._device_and_stream(x)
-    ws_ptr, ws_bytes, keep = _group_norm_workspace(workspace, batch, pixels, channels, groups, dtype, False, device)
     if wrapper.library().sideaware_group_norm_forward(
-            out_ptr, stats.data_ptr(), x_ptr, weight.data_ptr() if weight is not None else None, bias.data_ptr() if bias is not None else None,
-            batch, pixels, channels, groups, eps, act, dtype, weight_fp32, ws_ptr, ws_bytes, device, stream):
+            _aligned(out, "out"), stats.data_ptr(), _aligned(x, "x"), weight.data_ptr() if weight is not None else None,
+            bias.data_ptr() if bias is not None else None, batch, pixels, channels, groups, eps, act, dtype, weight_fp32, ws_ptr, ws_bytes, device, stream):
         _group_norm_failed("group_norm_forward")
     return out, stats
 
@@ -490,28 +554,27 @@ def group_norm_backward(dout, x, weight, bias, stats, groups: int, activation: s
     over samples and pixels (None where weight or bias is None).  ``stats`` is what the forward call returned.
     ``out`` may be ``dout``.  ``out``, ``dweight``, ``dbias`` and ``workspace`` are allocated unless given, as for the
     forward call."""
-    batch, pixels, channels, dtype, weight_fp32, act = _group_norm_shape(x, weight, bias, groups, activation)
-    assert dout.shape == x.shape and dout.dtype == x.dtype and dout.device == x.device, "the gradient is like the activation"
-    assert tuple(stats.shape) == (batch, groups, 2) and stats.dtype == torch.float32 and stats.is_contiguous() and stats.device == x.device, \
-        "stats are float32 (N, groups, 2)"
+    batch, pixels, channels, dtype, weight_fp32, act, need = _group_norm_call(x, weight, bias, groups, activation)
+    assert dout.shape == x.shape and dout.dtype == x.dtype and dout.get_device() == x.get_device(), "the gradient is like the activation"
+    _check_stats(stats, batch, groups, x)
     out = _like(out, x, "out")
-    grads = []
-    for given, param, name in ((dweight, weight, "dweight"), (dbias, bias, "dbias")):
-        assert given is None or param is not None, name + " goes with a parameter"
-        grads.append(None if param is None else _like(given, param, name))
-        assert param is None or grads[-1].is_contiguous(), name + " is contiguous"
-    dweight, dbias = grads
+    assert dweight is None or weight is not None, "dweight goes with a weight"
+    assert dbias is None or bias is not None, "dbias goes with a bias"
+    dweight = None if weight is None else _like(dweight, weight, "dweight")
+    dbias = None if bias is None else _like(dbias, bias, "dbias")
+    assert (dweight is None or dweight.is_contiguous()) and (dbias is None or dbias.is_contiguous()), "dweight and dbias are contiguous"
     if batch == 0:
-        for t in grads:
+        for t in (dweight, dbias):
             if t is not None:
                 t.zero_()
         return out, dweight, dbias
-    x_ptr, dout_ptr, out_ptr = wrapper._check(x, "x"), wrapper._check(dout, "dout"), wrapper._check(out, "out")
+    assert x.is_cuda, "x must be on the GPU"
+    ws_ptr, ws_bytes, keep = _workspace(workspace, need[1], x)
     device, stream = wrapper._device_and_stream(x)
-    ws_ptr, ws_bytes, keep = _group_norm_workspace(workspace, batch, pixels, channels, groups, dtype, True, device)
     if wrapper.library().sideaware_group_norm_backward(
-            out_ptr, dweight.data_ptr() if dweight is not None else None, dbias.data_ptr() if dbias is not None else None, dout_ptr, x_ptr,
-            weight.data_ptr() if weight is not None else None, bias.data_ptr() if bias is not None else None, stats.data_ptr(),
+            _aligned(out, "out"), dweight.data_ptr() if dweight is not None else None, dbias.data_ptr() if dbias is not None else None,
+            _aligned(dout, "dout"), _aligned(x, "x"), weight.data_ptr() if weight is not None else None,
+            bias.data_ptr() if bias is not None else None, stats.data_ptr(),
             batch, pixels, channels, groups, act, dtype, weight_fp32, ws_ptr, ws_bytes, device, stream):
         _group_norm_failed("group_norm_backward")
     return out, dweight, dbias
