@@ -538,16 +538,16 @@ def rope_axes_header(head_dim: int, sections, dtype: str = "bf16", half: bool = 
     over neighbouring ones.
 
     in0/out0: the activation, (tokens, heads, head_dim); in1: the fp32 table, (rows, head_dim/2, 2) of
-    (cos, sin), and in2, in3 the same pointer again (see below); the sideband pointer: int32
-    positions, (tokens, axes); the sideband value: :func:`rope_axes_sideband`.  A position outside
-    [0, rows) reads nothing of the table and makes the pairs of its axis NaN.
+    (cos, sin), less than 4 GiB; the sideband pointer: int32 positions, (tokens, axes); the sideband
+    value: :func:`rope_axes_sideband`.  A position outside [0, rows) reads nothing of the table and makes
+    the pairs of its axis NaN.
 
-    A lane rotates vec/2 pairs (4 of them for 16-bit types), whose cos and sin are 2 * vec/2 floats of
-    one row if all of them belong to one axis.  Where every lane's pairs do (sections of whole
-    multiples of vec/2 pairs, in blocks), one row is read, as by the ops with one position.
-    Elsewhere a lane reads its piece of the row of every axis, through in1, in2 and in3, and selects
-    pair by pair: rows are shared by all heads of a token and come out of the L1 cache, where the
-    additional reads cost little.
+    A lane rotates vec/2 pairs (4 of them for 16-bit types).  Where all of a lane's pairs belong to one axis
+    (sections of whole multiples of vec/2 pairs, in blocks) it reads one piece of one row, like the
+    ops with one position.  Elsewhere it reads each pair's (cos, sin) where that pair's row has it: reading its
+    piece of every axis' row and selecting took a third longer (4.4 against 6.0 TB/s for
+    19305 tokens of 48 fp32 heads of 128, dealt in turns).  Rows are shared by all heads of a token and come
+    out of the L1 cache.
     """
     if dtype not in _ROPE_HALF_TYPES:
         raise ValueError("dtype must be 'fp32', 'bf16' or 'fp16'")
@@ -572,11 +572,10 @@ def rope_axes_header(head_dim: int, sections, dtype: str = "bf16", half: bool = 
 
     name = "sideaware_rope_axes_%s_%s_%s_%s_d%d_%s" % ("bwd" if backward else "fwd", dtype, "half" if half else "pairs", order, head_dim,
                                                      "_".join(str(int(n)) for n in sections))
-    inputs = 1 if one_axis else axes                     # table rows a lane reads
     lines = ["#define KERNEL_NAME %s\n" % name,
-             "typedef %s o0;\ntypedef %s i0;\n" % (elem, elem), _UNUSED,
-             "".join("typedef %s i%d;\n" % ("float" if i <= inputs else "unused", i) for i in (1, 2, 3)),
-             "typedef unused o1, o2, o3;\n"]
+             "#define VECTOR_OP_GATHERS\n"
+             "typedef %s o0;\ntypedef %s i0;\ntypedef float i1;\n" % (elem, elem), _UNUSED,
+             "typedef unused o1, o2, o3, i2, i3;\n"]
     if unrolled is not None:
         lines.append("#define UNROLLED %d\n" % unrolled)
     lines.append("constexpr bool reverse_order = false;\n" + _evict([True]))
@@ -586,79 +585,64 @@ def rope_axes_header(head_dim: int, sections, dtype: str = "bf16", half: bool = 
         "constexpr int rope_axes = %d;\n"
         "constexpr int rope_vec = %d;           // elements per 16-byte vector\n"
         "constexpr int rope_unit = rope_vec / 2; // pairs a lane rotates\n"
-        "constexpr bool rope_half_split = %s;\n"
-        % (head_dim, pairs, axes, vec, "true" if half else "false"))
+        % (head_dim, pairs, axes, vec))
     if half:
         lines.append("constexpr int rope_partner_lanes = %d; // lanes between the two halves of a pair\n" % (pairs // vec))
     lines.append(
         "__device__ __forceinline__ void elementwise_op(size_t element_idx, int sideband,\n"
         "                               o0 &out0, o1 &out1, o2 &out2, o3 &out3,\n"
         "                               const i0 &in0, const i1 &in1, const i2 &in2, const i3 &in3) {}\n"
-        "// the axes of the pairs from `pair` on, two bits each (a lane's pairs never straddle a word)\n"
-        "__device__ __forceinline__ unsigned int rope_axis_code(int pair) {\n"
-        "    return (unsigned int)((%s) >> (2 * (pair %% 32)));\n"
-        "}\n"
-        "// the first pair this lane rotates, and the positions of its token\n"
-        "__device__ __forceinline__ int rope_first_pair(size_type elem) {\n"
-        "    const int in_head = (int)(elem %% rope_dim);\n"
-        "    if constexpr (rope_half_split) return in_head >= rope_half ? in_head - rope_half + rope_unit : in_head;\n"
-        "    else return in_head / 2;\n"
-        "}\n"
-        "__device__ __forceinline__ const int *rope_positions(size_type elem, const int *mem, int val) {\n"
-        "    const size_type token = elem / rope_dim / (size_type)((unsigned int)val & %du);\n"
-        "    return mem + token * rope_axes;\n"
-        "}\n"
-        "__device__ __forceinline__ bool rope_in_table(int position, int val) {\n"
-        "    return (unsigned int)position < ((unsigned int)val >> %d);\n"
-        "}\n"
-        % (code, ROPE_AXES_MAX_HEADS, _ROPE_AXES_HEADS_BITS))
-    # indices count groups of rope_vec floats: the (cos, sin) of rope_unit pairs
-    if one_axis:
-        lookup = ("    const int position = token[rope_axis_code(pair) & 3u];\n"
-                  "    idx_i1 = ((size_type)(rope_in_table(position, val) ? position : 0) * rope_half + pair) / rope_unit;\n"
-                  "    idx_i2 = 0;\n"
-                  "    idx_i3 = 0;\n")
-    else:
-        lookup = "".join(
-            "    idx_i%d = ((size_type)(rope_in_table(token[%d], val) ? token[%d] : 0) * rope_half + pair) / rope_unit;\n" % (a + 1, a, a)
-            for a in range(axes)) + "    idx_i3 = 0;\n" * (axes == 2)
-    lines.append(
-        "#define CUSTOM_IDX_FUNC\n"
-        "__device__ __forceinline__ bool indexing(size_type vec_idx, int vec_size,\n"
-        "                         size_type &idx_i0, size_type &idx_i1,\n"
-        "                         size_type &idx_i2, size_type &idx_i3, int* mem, int val) {\n"
-        "    const size_type elem = vec_idx * vec_size;\n"
-        "    const int pair = rope_first_pair(elem);\n"
-        "    const int *token = rope_positions(elem, mem, val);\n"
-        "    idx_i0 = vec_idx;\n" + lookup +
-        "    return false;\n"
-        "}\n")
+        "// indices are never negative, and unsigned numbers are divided faster\n"
+        "__device__ __forceinline__ unsigned int rope_index(int v) { return (unsigned int)v; }\n"
+        "__device__ __forceinline__ unsigned long long rope_index(long long v) { return (unsigned long long)v; }\n")
+    if half:
+        lines.append(_ROPE_PARTNER_WORD)
     angles = (
-        "    // the (cos, sin) of this lane's pairs\n"
-        "    const int pair = rope_first_pair(vec_idx * vec_size);\n"
-        "    const int *token = rope_positions(vec_idx * vec_size, sideband_memory, sideband_value);\n"
-        "    const unsigned int axis = rope_axis_code(pair);\n"
-        "    const float outside = __builtin_nanf(\"\");\n"
-        "    float cs[rope_vec];\n")
+        "    // the (cos, sin) of this lane's pairs, from the first of them\n"
+        "    const auto elem = rope_index(vec_idx * vec_size);\n"
+        "    const unsigned int in_head = (unsigned int)(elem %% rope_dim);\n"
+        "    const unsigned int pair = %s;\n"
+        "    const unsigned int rows = (unsigned int)sideband_value >> %d;\n"
+        "    const int *position = sideband_memory + (size_t)(elem / rope_dim / ((unsigned int)sideband_value & %du)) * rope_axes;\n"
+        "    // the axes of these pairs, two bits each (they never straddle a word)\n"
+        "    const unsigned int code = (unsigned int)((%s) >> (2 * (pair %% 32)));\n"
+        "    const char *table = (const char*)in1;\n"
+        "    float cs[rope_vec];\n"
+        % ("in_head >= rope_half ? in_head - rope_half + rope_unit : in_head" if half else "in_head / 2",
+           _ROPE_AXES_HEADS_BITS, ROPE_AXES_MAX_HEADS, code))
     if one_axis:
         angles += (
-            "    const bool ok = rope_in_table(token[axis & 3u], sideband_value);\n"
-            "    #pragma unroll\n"
-            "    for (int i = 0; i < rope_vec; i++) cs[i] = ok ? in1[i] : outside;\n")
+            "    const unsigned int row = (unsigned int)position[code & 3u];\n"
+            "    const bool ok = row < rows;\n"
+            "    __builtin_memcpy(cs, __builtin_assume_aligned(table + ((ok ? row : 0u) * rope_half + pair) * 8u, 16), sizeof cs);\n"
+            "    if (!ok) {\n"
+            "        #pragma unroll\n"
+            "        for (int i = 0; i < rope_vec; i++) cs[i] = __builtin_nanf(\"\");\n"
+            "    }\n")
     else:
-        angles += "".join("    const bool ok%d = rope_in_table(token[%d], sideband_value);\n" % (a, a) for a in range(axes))
-        pick = "ok0 ? in1[i] : outside"
+        angles += "".join("    const unsigned int row%d = (unsigned int)position[%d];\n" % (a, a) for a in range(axes))
+        pick = "row0"
         for a in range(1, axes):
-            pick = "a == %du ? (ok%d ? in%d[i] : outside) : (%s)" % (a, a, a + 1, pick)
+            pick = "a == %du ? row%d : %s" % (a, a, pick)
         angles += (
+            "    bool all = true;\n"
             "    #pragma unroll\n"
-            "    for (int i = 0; i < rope_vec; i++) {\n"
-            "        const unsigned int a = (axis >> (i / 2 * 2)) & 3u;\n"
-            "        cs[i] = %s;\n"
-            "    }\n" % pick)
+            "    for (int i = 0; i < rope_unit; i++) {\n"
+            "        const unsigned int a = (code >> (2 * i)) & 3u;\n"
+            "        const unsigned int row = %s;\n"
+            "        const bool ok = row < rows;\n"
+            "        all = all && ok;\n"
+            "        __builtin_memcpy(cs + 2 * i, __builtin_assume_aligned(table + ((ok ? row : 0u) * rope_half + pair + i) * 8u, 8), 8);\n"
+            "    }\n"
+            "    if (!all) {\n"
+            "        #pragma unroll\n"
+            "        for (int i = 0; i < rope_unit; i++) {\n"
+            "            const unsigned int a = (code >> (2 * i)) & 3u;\n"
+            "            if ((%s) >= rows) cs[2 * i] = cs[2 * i + 1] = __builtin_nanf(\"\");\n"
+            "        }\n"
+            "    }\n" % (pick, pick))
     if half:
         body = _ROPE_HALF_ROTATE.replace("@CS@", "cs").replace("@KEEP@", keep_sign).replace("@SEND@", send_sign)
-        lines.append(_ROPE_PARTNER_WORD)
     else:
         body = (
             "    #pragma unroll\n"

@@ -320,6 +320,8 @@ def _rope_axes_plan(shapes, out_shapes, dtypes, devices, freqs_shape, positions_
         raise TypeError("RoPE storage is float32, bfloat16 or float16")
     freqs_type, positions_type = dtypes[-2:]
     assert freqs_type == torch.float32 and len(freqs_shape) == 2 and freqs_shape[1] == head_dim, "the table is float32, (rows, head_dim)"
+    if freqs_shape[0] * freqs_shape[1] * 4 >= 1 << 32:
+        raise ValueError("the table of multi-axis RoPE is smaller than 4 GiB")
     assert positions_type == torch.int32, "positions are a contiguous int32 tensor"
     assert tuple(positions_shape) in ((B, T, len(sections)), (B * T, len(sections))), \
         "positions are (B, T, axes): one row of the table for each axis of every token"
@@ -349,7 +351,7 @@ def _rope_axes_many(tensors, freqs, positions, sections, half: bool, order: str,
     kid, sizes = plan
     if all(num_bytes for num_bytes, _ in sizes):
         table, where = _aligned(freqs, "freqs"), positions.data_ptr()
-        packed = b"".join([_SEGMENT.pack(num_bytes, _aligned(o, "out"), 0, 0, 0, _aligned(t, "x"), table, table, table, where, value)
+        packed = b"".join([_SEGMENT.pack(num_bytes, _aligned(o, "out"), 0, 0, 0, _aligned(t, "x"), table, 0, 0, where, value)
                            for t, o, (num_bytes, value) in zip(tensors, outs, sizes)])
         device, stream = wrapper._device_and_stream(freqs)
         wrapper.library().sideaware_elementwise_batch(kid, n, packed, device, stream)

@@ -113,7 +113,7 @@ def test_rope_axes_header_on_cpu(lib, tmp_path, dtype, d, sections, order, varia
             pos[0, 0] = 2 ** 31 - 1
             if tokens > 2:
                 pos[2, 0] = -1
-            got = run(exe, tmp_path, x, [table, table, table], pos, headers.rope_axes_sideband(heads, rows), grid, off).double().numpy()
+            got = run(exe, tmp_path, x, [table], pos, headers.rope_axes_sideband(heads, rows), grid, off).double().numpy()
             want = S.rope_axes(x.double().numpy(), table.double().numpy(), pos.numpy(), sections, False, order, backward)
             assert np.array_equal(np.isnan(got), np.isnan(want))
             # two products and a sum in fp32, then the storage; |x1 c| + |x2 s| <= |x| |table| maxima
