@@ -46,6 +46,7 @@ struct GnArgs {
     int per_group_log2;             // threads to a group where lanes' sums are added
     int param_x, param_blocks;      // workgroups of a row of the grid that add up dw and db, and how many do in all
     int weight_fp32, activation, finish;
+    int straddle;                   // a vector may hold channels of two groups
 };
 
 // The values of a vector stay packed in whole words until they are used: as an array of 16-bit values each of
@@ -422,6 +423,86 @@ __device__ __forceinline__ void forward_stats(const GnArgs& a, const Place& q, l
     __syncthreads();
 }
 
+// What becomes of a group's two sums as soon as one thread has them, where nothing else adds to them: a chunk's go to
+// the workspace, a sample's become its statistics.
+template<int MODE>
+__device__ __forceinline__ void forward_emit(const GnArgs& a, const Place& q, long long n, int at, double t1, double t2, float (*stat)[2]) {
+    if constexpr (MODE == kSums) {
+        double2* part = (double2*)a.group_part + ((n * gridDim.y + q.slab) * a.chunks + q.chunk) * a.slab_groups;
+        part[at] = {t1, t2};
+    } else {
+        float s[2];
+        write_stats(s, t1 * a.inv_count, t2 * a.inv_count, a.eps);
+        *(float2*)stat[at] = {s[0], s[1]};
+        ((float2*)a.stats)[n * a.groups + q.first_group + at] = {s[0], s[1]};
+    }
+}
+
+// forward_group_sums() for one slice and groups no narrower than a vector, which then touches one group, or two where
+// groups are no multiple of it (`straddle`): nothing is accumulated in between, so each group's threads pass its sums on.
+template<int VEC, int MODE>
+__device__ __forceinline__ void forward_group_sums_at_once(const GnArgs& a, const Place& q, long long n, int count, const int (&g)[VEC],
+                                                           const float (&pivot)[VEC], const float (&s1)[VEC], const float (&s2)[VEC], double* lds,
+                                                           float (*stat)[2]) {
+    const int slots = a.straddle ? 2 : 1;
+    double2* lanes = (double2*)lds;                               // [row][vector][slot]
+    if (q.ty < a.rows) {
+        double2* to = lanes + (q.ty * a.slice_vectors + q.tx) * slots;
+        auto leave = [&](int slot, float f1, float f2, float p, int values) {
+            const double dp = p, m = values, df = f1;
+            double2 t = {df + m * dp, f2 + dp * (2.0 * df + m * dp)};
+            if (values == 0) t = {0, 0};
+            to[slot] = t;
+        };
+        float f1 = 0, f2 = 0;
+        if (!a.straddle) {
+            #pragma unroll
+            for (int j = 0; j < VEC; j++) { f1 += s1[j]; f2 += s2[j]; }
+            leave(0, f1, f2, pivot[0], VEC * count);
+        } else {
+            float h1 = 0, h2 = 0;
+            int in = 0;
+            #pragma unroll
+            for (int j = 0; j < VEC; j++) {
+                const bool first = g[j] == g[0];
+                f1 += first ? s1[j] : 0.0f;
+                f2 += first ? s2[j] : 0.0f;
+                h1 += first ? 0.0f : s1[j];
+                h2 += first ? 0.0f : s2[j];
+                in += first ? count : 0;
+            }
+            leave(0, f1, f2, pivot[0], in);
+            leave(1, h1, h2, pivot[VEC - 1], VEC * count - in);
+        }
+    }
+    __syncthreads();
+    const int per = 1 << a.per_group_log2;
+    const int first = (int)threadIdx.x >> a.per_group_log2, part = (int)threadIdx.x & (per - 1), step = (int)blockDim.x >> a.per_group_log2;
+    const int end = q.end_vector - q.first_vector;
+    for (int base = 0; base < q.groups; base += step) {
+        const int at = base + first;
+        double t1 = 0, t2 = 0;
+        if (at < q.groups) {
+            const int c0 = at * a.group_channels, lo = c0 / VEC, vectors = min((c0 + a.group_channels - 1) / VEC + 1, end) - lo;
+            const float inv = __builtin_amdgcn_rcpf((float)vectors);
+            #pragma unroll 2
+            for (int e = part; e < vectors * a.rows; e += per) {
+                int row = (int)((float)e * inv);                  // e / vectors, off by one at most
+                if (row * vectors > e) row--;
+                if ((row + 1) * vectors <= e) row++;
+                const int w = lo + e - row * vectors;
+                const double2 t = lanes[(row * a.slice_vectors + w) * slots + (w * VEC < c0 ? 1 : 0)];
+                t1 += t.x;
+                t2 += t.y;
+            }
+        }
+        t1 = add_over(t1, a.per_group_log2);
+        t2 = add_over(t2, a.per_group_log2);
+        if (at < q.groups && part == 0) forward_emit<MODE>(a, q, n, at, t1, t2, stat);
+    }
+    __syncthreads();
+}
+
 // two floats of each of the slab's groups
 __device__ __forceinline__ void load_stats(const float* from, const GnArgs& a, const Place& q, long long n, float (*stat)[2]) {
     const float* at = from + (n * a.groups + q.first_group) * 2;
@@ -471,10 +552,13 @@ __device__ __forceinline__ void forward_apply(const GnArgs& a, const Lane<T, VEC
 }
 
 
-// ONE: a workgroup has one sample and its slab is one slice, as nearly always; the loops over them then go, and with
-// them the registers that what they repeat would hold.
-template<typename T, int VEC, int MODE, bool ONE>
+// kOne: a workgroup has one sample and its slab is one slice, as nearly always; the loops over them then go, and with
+// them the registers that what they repeat would hold.  kOneWide: groups are no narrower than a vector, too.
+enum Kind { kLoops, kOne, kOneWide };
+
+template<typename T, int VEC, int MODE, int KIND>
 __global__ __launch_bounds__(kGroupNormMaxThreads, 4) void group_norm_forward(GnArgs a) {
+    constexpr bool ONE = KIND != kLoops, AT_ONCE = KIND == kOneWide;
     extern __shared__ double lds[];
     __shared__ double sums[kGroupNormMaxSlabGroups][2];
     __shared__ float stat[kGroupNormMaxSlabGroups][2];
@@ -498,7 +582,7 @@ __global__ __launch_bounds__(kGroupNormMaxThreads, 4) void group_norm_forward(Gn
             }
         }
         if constexpr (!applies_only(MODE)) {
-            clear_sums(q, sums);
+            if constexpr (!AT_ONCE) clear_sums(q, sums);
             int v0 = q.first_vector;
             do {
                 const Lane<T, VEC> lane(a, q, n, v0);
@@ -516,16 +600,17 @@ __global__ __launch_bounds__(kGroupNormMaxThreads, 4) void group_norm_forward(Gn
                         forward_lane_sums<T, VEC, B>(a, lane, pre, g, pivot, s1, s2);
                     }
                 }
-                forward_group_sums<VEC>(a, q, v0, lane.count, g, pivot, s1, s2, lds, sums);
+                if constexpr (AT_ONCE) forward_group_sums_at_once<VEC, MODE>(a, q, n, lane.count, g, pivot, s1, s2, lds, stat);
+                else forward_group_sums<VEC>(a, q, v0, lane.count, g, pivot, s1, s2, lds, sums);
                 v0 += a.slice_vectors;
             } while (!ONE && v0 < q.end_vector);
         }
         if constexpr (MODE == kSums) {
-            write_part(a, q, n, sums);
+            if constexpr (!AT_ONCE) write_part(a, q, n, sums);
         } else {
             if (applies_only(MODE) && a.finish) {
                 load_stats(a.stats, a, q, n, stat);
-            } else {
+            } else if constexpr (applies_only(MODE) || !AT_ONCE) {
                 if constexpr (applies_only(MODE)) gather_chunks(a, q, n, lds, sums);
                 forward_stats(a, q, n, sums, stat, q.chunk == 0);
             }
@@ -684,9 +769,9 @@ __device__ __forceinline__ void backward_lane_sums(const GnArgs& a, const Place&
 
 // Adds the lanes' sums up to channels (for the gradients of weight and bias, into `row` of the workspace) and
 // those, weighted, to the slab's groups.
-template<typename T, int VEC>
-__device__ __forceinline__ void backward_group_sums(const GnArgs& a, const Place& q, int v0, bool on, const float (&s1)[VEC], const float (&s2)[VEC],
-                                                    double* lds, double (*sums)[2], long long row, bool add_to_row) {
+template<typename T, int VEC, int MODE, bool ONE>
+__device__ __forceinline__ void backward_group_sums(const GnArgs& a, const Place& q, long long n, int v0, bool on, const float (&s1)[VEC], const float (&s2)[VEC],
+                                                    double* lds, double (*sums)[2], float (*stat)[2], long long row, bool add_to_row) {
     const int slice_channels = a.slice_vectors * VEC;
     const int c0 = v0 * VEC, here = min(v0 + a.slice_vectors, q.end_vector) * VEC - c0;      // channels of the slice
     float* lanes = (float*)lds;                                   // [which][row][channel of the slice]
@@ -732,8 +817,15 @@ __device__ __forceinline__ void backward_group_sums(const GnArgs& a, const Place
         t1 = add_over(t1, a.per_group_log2);
         t2 = add_over(t2, a.per_group_log2);
         if (at < q.groups && part == 0) {
-            sums[at][0] += t1;
-            sums[at][1] += t2;
+            if constexpr (!ONE) {
+                sums[at][0] += t1;
+                sums[at][1] += t2;
+            } else if constexpr (MODE == kSums) {
+                ((double2*)a.group_part)[((n * gridDim.y + q.slab) * a.chunks + q.chunk) * a.slab_groups + at] = {t1, t2};
+            } else {
+                stat[at][0] = (float)(t1 * a.inv_count);
+                stat[at][1] = (float)(t2 * a.inv_count);
+            }
         }
     }
     __syncthreads();
@@ -856,7 +948,7 @@ __global__ __launch_bounds__(kGroupNormMaxThreads, 4) void group_norm_backward(G
             }
         }
         if constexpr (!applies_only(MODE)) {
-            clear_sums(q, sums);
+            if constexpr (!ONE) clear_sums(q, sums);
             int v0 = q.first_vector;
             do {
                 const Lane<T, VEC> lane(a, q, n, v0);
@@ -879,16 +971,16 @@ __global__ __launch_bounds__(kGroupNormMaxThreads, 4) void group_norm_backward(G
                         sum(px, pg);
                     }
                 }
-                backward_group_sums<T, VEC>(a, q, v0, lane.count != 0, s1, s2, lds, sums, q.n * a.chunks + q.chunk, n != q.n);
+                backward_group_sums<T, VEC, MODE, ONE>(a, q, n, v0, lane.count != 0, s1, s2, lds, sums, stat, q.n * a.chunks + q.chunk, n != q.n);
                 v0 += a.slice_vectors;
             } while (!ONE && v0 < q.end_vector);
         }
         if constexpr (MODE == kSums) {
-            write_part(a, q, n, sums);
+            if constexpr (!ONE) write_part(a, q, n, sums);
         } else {
             if (applies_only(MODE) && a.finish) {
                 load_stats(a.means, a, q, n, stat);
-            } else {
+            } else if constexpr (applies_only(MODE) || !ONE) {
                 if constexpr (applies_only(MODE)) gather_chunks(a, q, n, lds, sums);
                 for (int g = (int)threadIdx.x; g < q.groups; g += (int)blockDim.x) {
                     stat[g][0] = (float)(sums[g][0] * a.inv_count);
@@ -948,22 +1040,23 @@ GnArgs args_of(const GroupNormCall& c) {
     a.last_chunk = a.last_pixels ? (int)((runs - 1) % p.chunks) : -1;
     while (a.per_group_log2 < 6 && (p.slab_groups << (a.per_group_log2 + 1)) <= p.threads) a.per_group_log2++;
     a.weight_fp32 = c.weight_fp32; a.activation = c.activation; a.finish = p.finish;
+    a.straddle = p.group_channels % p.vec != 0;
     return a;
 }
 
 dim3 grid_of(const GroupNormPlan& p) { return dim3((unsigned)p.chunks, (unsigned)p.slabs, (unsigned)p.batch_blocks); }
 dim3 finish_grid_of(const GroupNormPlan& p) { return dim3((unsigned)(p.slab_groups + 3) / 4, (unsigned)p.slabs, (unsigned)p.batch_blocks); }
 
-template<typename T, int VEC, bool ONE>
+template<typename T, int VEC, int KIND>
 hipError_t forward_of(const GroupNormCall& c, hipStream_t stream) {
     const GroupNormPlan& p = c.plan;
     const GnArgs a = args_of(c);
     const dim3 grid = grid_of(p), block((unsigned)p.threads);
     if (p.chunks == 1) {
-        group_norm_forward<T, VEC, kBoth, ONE><<<grid, block, p.lds_bytes, stream>>>(a);
+        group_norm_forward<T, VEC, kBoth, KIND><<<grid, block, p.lds_bytes, stream>>>(a);
         return hipGetLastError();
     }
-    group_norm_forward<T, VEC, kSums, ONE><<<grid, block, p.lds_bytes, stream>>>(a);
+    group_norm_forward<T, VEC, kSums, KIND><<<grid, block, p.lds_bytes, stream>>>(a);
     hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
     if (p.finish) {
@@ -971,8 +1064,8 @@ hipError_t forward_of(const GroupNormCall& c, hipStream_t stream) {
         err = hipGetLastError();
         if (err != hipSuccess) return err;
     }
-    if (p.stream) group_norm_forward<T, VEC, kApplyStream, ONE><<<grid, block, p.lds_bytes, stream>>>(a);
-    else group_norm_forward<T, VEC, kApply, ONE><<<grid, block, p.lds_bytes, stream>>>(a);
+    if (p.stream) group_norm_forward<T, VEC, kApplyStream, KIND == kLoops ? kLoops : kOne><<<grid, block, p.lds_bytes, stream>>>(a);
+    else group_norm_forward<T, VEC, kApply, KIND == kLoops ? kLoops : kOne><<<grid, block, p.lds_bytes, stream>>>(a);
     return hipGetLastError();
 }
 
@@ -1012,10 +1105,12 @@ template<typename T, int VEC>
 hipError_t launch_of(const GroupNormCall& c, bool backward, hipStream_t stream) {
     // (instantiated for full vectors only: the others are built once, with the loops)
     if constexpr (sizeof(T) * VEC == 16) {
-        if (c.plan.batch_blocks == c.batch && c.plan.slab_vectors <= c.plan.slice_vectors)
-            return backward ? backward_of<T, VEC, true>(c, stream) : forward_of<T, VEC, true>(c, stream);
+        if (c.plan.batch_blocks == c.batch && c.plan.slab_vectors <= c.plan.slice_vectors) {
+            if (backward) return backward_of<T, VEC, true>(c, stream);
+            return c.plan.group_channels >= VEC ? forward_of<T, VEC, kOneWide>(c, stream) : forward_of<T, VEC, kOne>(c, stream);
+        }
     }
-    return backward ? backward_of<T, VEC, false>(c, stream) : forward_of<T, VEC, false>(c, stream);
+    return backward ? backward_of<T, VEC, false>(c, stream) : forward_of<T, VEC, kLoops>(c, stream);
 }
 
 template<typename T>
