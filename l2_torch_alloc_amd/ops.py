@@ -8,6 +8,7 @@ even and sin at odd columns.
 """
 from __future__ import annotations
 
+import ctypes
 import math
 import os
 import struct
@@ -147,8 +148,15 @@ def rope_backward_heads(dout, freqs, out=None, positions=None):
     return _rope(dout, freqs, out, 0, 0, "heads", True, positions)
 
 
-# ``sideaware_segment`` of include/sideaware.h: num_bytes, out[4], in[4], sideband_memory, sideband_value
+class _Segment(ctypes.Structure):
+    """``sideaware_segment`` of include/sideaware.h."""
+    _fields_ = [("num_bytes", ctypes.c_size_t), ("out", ctypes.c_void_p * 4), ("inp", ctypes.c_void_p * 4),
+                ("sideband_memory", ctypes.c_void_p), ("sideband_value", ctypes.c_int)]
+
+
+# The same layout, filled in one step (field by field costs a small launch several times its C call).
 _SEGMENT = struct.Struct("=Q4Q4QQi4x")
+assert _SEGMENT.size == ctypes.sizeof(_Segment)
 
 
 def elementwise_batch(kernel_id: int, segments) -> None:
@@ -349,15 +357,12 @@ def _rope_axes_many(tensors, freqs, positions, sections, half: bool, order: str,
         plan = _keep_plan(key, _rope_axes_plan(shapes[:n], shapes[n:-2], dtypes, devices, freqs.shape, positions.shape,
                                                tuple(int(s) for s in sections), bool(half), order, backward))
     kid, sizes = plan
-    if all(num_bytes for num_bytes, _ in sizes):
+    if sizes[0][0]:                                            # all have elements, or none
         table, where = _aligned(freqs, "freqs"), positions.data_ptr()
         packed = b"".join([_SEGMENT.pack(num_bytes, _aligned(o, "out"), 0, 0, 0, _aligned(t, "x"), table, 0, 0, where, value)
                            for t, o, (num_bytes, value) in zip(tensors, outs, sizes)])
         device, stream = wrapper._device_and_stream(freqs)
         wrapper.library().sideaware_elementwise_batch(kid, n, packed, device, stream)
-    elif any(num_bytes for num_bytes, _ in sizes):             # tensors without heads among others
-        some = [i for i in range(n) if sizes[i][0]]
-        _rope_axes_many([tensors[i] for i in some], freqs, positions, sections, half, order, backward, [outs[i] for i in some])
     return outs
 
 
@@ -484,6 +489,8 @@ def _group_norm_call(x: torch.Tensor, weight, bias, groups: int, activation: str
 def _may_allocate(what: str) -> None:
     """Under this library's allocator, memory that is allocated while a stream is being captured goes back to
     the pool when the tensor dies, while the graph still writes it."""
+    if torch.compiler.is_compiling():                          # the tracer allocates
+        return
     if wrapper._allocator_installed and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("under stream capture pass %s: the graph needs memory that outlives it" % what)
 

@@ -113,7 +113,8 @@ SHAPES = [
     # channel per group, several samples per workgroup, wide rows cut into slabs and slices
     (1, 1, 8, 1), (2, 1, 64, 8), (3, 5, 30, 10), (2, 64, 1280, 32), (1, 7, 33, 11), (2, 100, 7, 1), (4, 9, 48, 48), (3, 1024, 24, 4),
     (1, 4096, 320, 32), (2, 5003, 96, 8), (1, 3000, 1029, 3), (2, 333, 8200, 1), (1, 2, 20000, 4), (1, 40000, 1, 1), (700, 3, 16, 2),
-    (1, 30011, 40, 4), (2, 2048, 2560, 32), (5000, 1, 8, 2), (1, 70000, 12, 3)]
+    (1, 30011, 40, 4), (2, 2048, 2560, 32), (5000, 1, 8, 2), (1, 70000, 12, 3),
+    (2, 6001, 128, 32), (1, 20000, 64, 64), (3, 1369, 1152, 24), (20, 1024, 64, 4)]
 
 
 @pytest.mark.parametrize("N,P,C,G", SHAPES)
@@ -138,6 +139,9 @@ def test_group_norm(sa, N, P, C, G):
         g3 = gd.clone()
         again = ops.group_norm_backward(g3, xd, wd, bd, stats, G, activation=activation, out=g3)
         assert again[0] is g3 and all(torch.equal(p, q) for p, q in zip(got, again))
+        x4 = xd.clone()
+        again = ops.group_norm_backward(gd, x4, wd, bd, stats, G, activation=activation, out=x4)
+        assert again[0] is x4 and all(torch.equal(p, q) for p, q in zip(got, again))
     no_error(sa)
 
 

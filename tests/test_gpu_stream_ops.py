@@ -284,3 +284,17 @@ def test_empty_and_refused(sa):
     lib.sideaware_clear_error()
     torch.cuda.synchronize()
     assert bool((x == 1).all())
+
+
+def test_dropout_under_torch_compile(sa):
+    from l2_torch_alloc_amd import ops
+
+    @torch.compile(fullgraph=True)
+    def step(x, seed, residual):
+        return ops.dropout_forward(x * 2, 0.25, seed, residual=residual) + 1
+
+    x, r = torch.randn(64, 96, device="cuda"), torch.randn(64, 96, device="cuda")
+    seed = torch.tensor([3, 1]).cuda()
+    want = ops.dropout_forward(x * 2, 0.25, seed, residual=r) + 1
+    assert torch.equal(step(x, seed, r), want)
+    no_error(sa)
