@@ -5,8 +5,14 @@
 //   dz = dout act'(z);  db = sum dz,  dw = sum dz h  (over samples and pixels)
 //   dx = r (w dz - mean_g(w dz) - h mean_g(w dz h))  (means over the (sample, group))
 //
-// Bound by memory: the array must be read before the first value of its output is known, so it is read
-// twice, the second time out of the caches where it fits them (a workgroup's own, or the Infinity Cache).
+// Bound by memory: the array must be read before the first value of its output is known, so it is read twice, the
+// second time out of the caches where it fits them (a workgroup's own, or the Infinity Cache).  Forward, bf16 with SiLU
+// and fp32 parameters: 512x512 pixels of 256 channels (134 MB) 73 us, 3.7 TB/s of what has to be read and written, of
+// which 25 us for the sums (memory), 5 for adding the chunks' sums and 43 for the values (6.2 TB/s of what they read and
+// write); 8 samples of 64x64 pixels of 320 channels (21 MB) 17 us, 8 and 9 for the two launches, of which about 3 us each
+// go into adding sums up across lanes and workgroups.  Backward with SiLU is bound by the vector ALU too: 21 issue
+// slots a value for the sums, of which an exponential and a reciprocal take eight; 16 samples of 32x32 pixels of 640
+// channels (21 MB) 28 us, 2.2 TB/s.
 //
 // A lane keeps one vector of channels and walks pixels, so all accesses of a wave are runs of whole
 // vectors and its sums are per channel, in registers; whatever the number of channels in a group is,
@@ -282,7 +288,9 @@ constexpr bool applies_only(int mode) { return mode == kApply || mode == kApplyS
 
 // All workgroups start together and would stay in step: every lane waiting for its batch of loads, then every lane
 // computing and the memory idle.  So the load that follows on a pixel's heels is issued where that pixel's registers are
-// free, and this keeps the compiler from collecting the loads again.
+// free, and this keeps the compiler from collecting the loads again (64 samples of 256 pixels of 512 channels: 17 us, 19
+// in batches).  The loops are not unrolled further and their last steps are loops of their own: with fewer instructions to
+// fetch, a call of few values is faster (16 samples of one pixel: 6.7 us with batches of 2, 7.8 with batches of 6).
 __device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
 
 // ---- forward -----------------------------------------------------------------------------------
