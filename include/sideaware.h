@@ -135,7 +135,8 @@ void sideaware_elementwise_batch(int kernel_id, int num_segments, const sideawar
  * bias 0.  activation: 0 none, 1 SiLU (z / (1 + e^-z)).  stats is (batch, groups, 2) fp32, (mean, r):
  * written by the forward call, read by the backward one.  All sums are kept in 32 bits or more, in an
  * order that does not depend on the run: the same call gives the same bits.
- * out may be x, and dx may be dout (or x).  dweight and dbias may be null.
+ * out may be x, and dx may be dout (or x); otherwise what a call writes shares no memory with its other
+ * arrays (refused).  dweight and dbias may be null.
  * The workspace holds partial sums between a call's launches: at least sideaware_group_norm_workspace()
  * bytes (0 where the call needs none, and on an error), with nothing to be cleared; calls that may overlap
  * (on different streams, or captured into different graphs) each need their own.

@@ -1246,6 +1246,19 @@ size_t sideaware_group_norm_workspace(long long batch, long long pixels, int cha
                ? plan.workspace_bytes : 0;
 }
 
+// Of what a call writes (its first `outputs` arrays) no part is part of another array of the call: workgroups finish
+// in any order.  The first may be an input itself, value for value.
+struct GroupNormArray { const void* at; size_t bytes; bool may_be_first; };
+static bool group_norm_arrays_overlap(const GroupNormArray* arrays, int outputs, int count) {
+    for (int o = 0; o < outputs; o++)
+        for (int i = o + 1; i < count; i++) {
+            const GroupNormArray &w = arrays[o], &r = arrays[i];
+            if (!w.at || !r.at || (o == 0 && r.may_be_first && w.at == r.at)) continue;
+            if ((uintptr_t)w.at < (uintptr_t)r.at + r.bytes && (uintptr_t)r.at < (uintptr_t)w.at + w.bytes) return true;
+        }
+    return false;
+}
+
 static int run_group_norm(const char* what, bool backward, GroupNormCall& call, int dtype, int weight_fp32, void* workspace, size_t workspace_bytes,
                           int device, sideaware_stream_t stream) {
     DeviceContext* ctx = plan_group_norm_call(what, call.batch, call.pixels, call.channels, call.groups, dtype, backward, device, &call.plan);
@@ -1268,6 +1281,17 @@ static int run_group_norm(const char* what, bool backward, GroupNormCall& call, 
     }
     call.type = dtype;
     call.weight_fp32 = weight_fp32 != 0 || dtype == kGroupNormFp32;
+    const size_t bytes = (size_t)(call.batch * call.pixels) * call.channels * group_norm_element_bytes(dtype);
+    const size_t param_bytes = (size_t)call.channels * (call.weight_fp32 ? 4 : group_norm_element_bytes(dtype));
+    const size_t stats_bytes = (size_t)call.batch * call.groups * 2 * sizeof(float);
+    const GroupNormArray arrays[] = {                             // stats are written forward and read backward
+        {call.out, bytes, false}, {call.dweight, param_bytes, false}, {call.dbias, param_bytes, false},
+        {workspace, call.plan.workspace_bytes, false}, {call.stats, stats_bytes, false},
+        {call.x, bytes, true}, {call.dout, bytes, true}, {call.weight, param_bytes, false}, {call.bias, param_bytes, false}};
+    if (group_norm_arrays_overlap(arrays, backward ? 4 : 5, 9)) {
+        set_error("%s: an output overlaps another array of the call", what);
+        return -1;
+    }
     call.workspace = workspace;
     ScopedDevice guard(ctx->device);
     const int err = backward ? launch_group_norm_backward(call, stream) : launch_group_norm_forward(call, stream);

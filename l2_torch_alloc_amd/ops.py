@@ -318,6 +318,13 @@ def _aligned(t: torch.Tensor, name: str) -> int:
     return ptr
 
 
+def _refuse_overlap(out: int, out_bytes: int, array: int, array_bytes: int) -> None:
+    """Of an output and another array of a launch, by address: workgroups finish in any order, so an output may
+    be an input itself, element for element, but not share part of another array's memory."""
+    if out < array + array_bytes and array < out + out_bytes:
+        raise ValueError("an output overlaps another array of the call")
+
+
 def _rope_axes_plan(shapes, out_shapes, dtypes, devices, freqs_shape, positions_shape, sections, half, order, backward):
     """The kernel and, for each tensor with elements, its bytes and sideband value."""
     first = shapes[0]
@@ -359,8 +366,17 @@ def _rope_axes_many(tensors, freqs, positions, sections, half: bool, order: str,
     kid, sizes = plan
     if sizes[0][0]:                                            # all have elements, or none
         table, where = _aligned(freqs, "freqs"), positions.data_ptr()
-        packed = b"".join([_SEGMENT.pack(num_bytes, _aligned(o, "out"), 0, 0, 0, _aligned(t, "x"), table, 0, 0, where, value)
-                           for t, o, (num_bytes, value) in zip(tensors, outs, sizes)])
+        arrays = [(_aligned(o, "out"), _aligned(t, "x"), size) for t, o, (size, _) in zip(tensors, outs, sizes)]
+        for i, (out, inp, size) in enumerate(arrays):
+            if out != inp:
+                _refuse_overlap(out, size, inp, size)
+            for other_out, other_inp, other_size in arrays[:i]:
+                _refuse_overlap(out, size, other_out, other_size)
+                _refuse_overlap(out, size, other_inp, other_size)
+                if out != inp:
+                    _refuse_overlap(other_out, other_size, inp, size)
+        packed = b"".join([_SEGMENT.pack(size, out, 0, 0, 0, inp, table, 0, 0, where, value)
+                           for (out, inp, size), (_, value) in zip(arrays, sizes)])
         device, stream = wrapper._device_and_stream(freqs)
         wrapper.library().sideaware_elementwise_batch(kid, n, packed, device, stream)
     return outs
@@ -369,7 +385,8 @@ def _rope_axes_many(tensors, freqs, positions, sections, half: bool, order: str,
 def rope_axes_forward_many(tensors, freqs, positions, sections, half: bool = False, order: str = "blocks", outs=None):
     """RoPE with a position of 1 to 3 axes (the time, height and width of an image's or video's patch) of
     several (B, T, heads, head_dim) tensors in ONE launch: q and k of a grouped-query model (different
-    head counts, same B, T, head_dim and dtype).  In place unless ``outs`` is given; returns the outputs.
+    head counts, same B, T, head_dim and dtype).  In place unless ``outs`` is given; returns the outputs.  An
+    output is its own tensor or shares no memory with any other.
 
     ``freqs``: the (rows, head_dim) fp32 table of the ops with one position (``freqs_cis_table``, or
     ``freqs_cis_axes_table`` for axes with frequencies of their own), with a row for every position that
@@ -415,16 +432,19 @@ def _dropout(x: torch.Tensor, p: float, seed: torch.Tensor, residual: Optional[t
         assert residual.shape == x.shape and residual.dtype == x.dtype and residual.get_device() == device, "the residual is like the activation"
     out = _like(out, x, "out")
     if x.numel():
-        kid = _kernel_ids.get(("dropout", (dtype, residual is not None), ()))
-        if kid is None or torch.compiler.is_compiling():
-            kid = _kernel("dropout", (dtype, residual is not None))
-            _elementwise(kid, out, None, None, None, x, residual, None, None, seed, threshold, 0, 0)
+        if torch.compiler.is_compiling():
+            _elementwise(_kernel("dropout", (dtype, residual is not None)), out, None, None, None, x, residual, None, None, seed, threshold, 0, 0)
         else:
             assert x.is_cuda, "x must be on the GPU"
+            kid = _kernel("dropout", (dtype, residual is not None))
+            size, to, first = x.numel() * x.element_size(), _aligned(out, "out"), _aligned(x, "x")
+            second = 0 if residual is None else _aligned(residual, "residual")
+            if to != first:
+                _refuse_overlap(to, size, first, size)
+            if second and to != second:
+                _refuse_overlap(to, size, second, size)
             device, stream = wrapper._device_and_stream(x)
-            wrapper.library().sideaware_elementwise(kid, x.numel() * x.element_size(), _aligned(out, "out"), 0, 0, 0, _aligned(x, "x"),
-                                                    0 if residual is None else _aligned(residual, "residual"), 0, 0, seed.data_ptr(), threshold,
-                                                    0, 0, device, stream)
+            wrapper.library().sideaware_elementwise(kid, size, to, 0, 0, 0, first, second, 0, 0, seed.data_ptr(), threshold, 0, 0, device, stream)
     return out
 
 
@@ -434,7 +454,7 @@ def dropout_forward(x, p: float, seed, residual=None, out=None):
     is computed from the element's index and ``seed``, an int64 device tensor (seed, offset), and never
     stored: pass the same two to :func:`dropout_backward`.  A launch captured into a graph reads the
     tensor at every replay, so advancing the offset in place gives each replay a new mask.
-    ``x`` may have any number of elements.  ``out`` may be ``x`` or ``residual``."""
+    ``x`` may have any number of elements.  ``out`` may be ``x`` or ``residual``, but not overlap them otherwise."""
     return _dropout(x, p, seed, residual, out)
 
 

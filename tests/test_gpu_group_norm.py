@@ -312,3 +312,40 @@ def test_refused(sa):
     lib.sideaware_clear_error()
     torch.cuda.synchronize()
     assert bool((y == 5).all())
+
+
+def test_overlapping_arrays_are_refused(sa):
+    """An output may be x or dout, but no other arrays of a call may share memory with what it writes."""
+    from l2_torch_alloc_amd import ops
+    lib = sa.library()
+    n, pixels, channels = 1, 9000, 16
+    count = n * pixels * channels
+    buf = torch.ones(2 * count + 64, device="cuda")
+    shape = (n, pixels, channels)
+    x, behind, dout = buf[:count].view(shape), buf[32:count + 32].view(shape), buf[count + 64:].view(shape)
+    w, b = torch.ones(channels, device="cuda"), torch.zeros(channels, device="cuda")
+    stats = torch.ones(n, 4, 2, device="cuda")
+    other = torch.empty_like(x)
+    need = ops.group_norm_workspace(x, 4, backward=True)
+    assert need > 0
+    inside = x.view(-1)[:(need + 3) // 4]
+    for call in (lambda: ops.group_norm_forward(x, w, b, 4, out=behind, stats=stats),
+                 lambda: ops.group_norm_forward(x, w, b, 4, out=other, stats=x.view(-1)[:8].view(1, 4, 2)),
+                 lambda: ops.group_norm_forward(x, w, b, 4, out=other, stats=stats, workspace=inside),
+                 lambda: ops.group_norm_forward(x, x.view(-1)[:16], b, 4, out=x, stats=stats),
+                 lambda: ops.group_norm_backward(dout, x, w, b, stats, 4, out=behind),
+                 lambda: ops.group_norm_backward(dout, x, w, b, stats, 4, out=other, dweight=w),
+                 lambda: ops.group_norm_backward(dout, x, w, b, stats, 4, out=other, dweight=b),
+                 lambda: ops.group_norm_backward(dout, x, w, b, stats, 4, out=other, dweight=other.view(-1)[:16]),
+                 lambda: ops.group_norm_backward(dout, x, w, b, stats, 4, out=other, dweight=buf[-16:], dbias=buf[-16:]),
+                 lambda: ops.group_norm_backward(dout, x, w, b, stats, 4, out=other, workspace=inside)):
+        with pytest.raises(RuntimeError, match="overlap"):
+            call()
+        lib.sideaware_clear_error()
+    torch.cuda.synchronize()
+    assert bool((buf == 1).all()) and bool((w == 1).all()) and bool((b == 0).all()) and bool((stats == 1).all())
+    # one tensor as input, gradient and weight and bias of another call is all right
+    want = ops.group_norm_backward(x, x, w, w, stats, 4)
+    have = ops.group_norm_backward(x, x, w, w, stats, 4, out=x)
+    assert all(torch.equal(h, t) for h, t in zip(have, want))
+    no_error(sa)

@@ -298,3 +298,34 @@ def test_dropout_under_torch_compile(sa):
     want = ops.dropout_forward(x * 2, 0.25, seed, residual=r) + 1
     assert torch.equal(step(x, seed, r), want)
     no_error(sa)
+
+
+def test_overlapping_arrays_are_refused(sa):
+    """An output may be its own input, but not share memory with another array of the launch."""
+    from l2_torch_alloc_amd import ops
+    seed, sections = torch.tensor([3, 1]).cuda(), (16, 16)
+    table = ops.freqs_cis_axes_table(sections, 8, 10000.0).cuda()
+    pos = torch.zeros(2, 5, 2, dtype=torch.int32, device="cuda") + 3
+    shape, n = (2, 5, 3, 64), 2 * 5 * 3 * 64
+    buf = torch.ones(4 * n, device="cuda")
+    x, behind, apart = buf[:n].view(shape), buf[16:n + 16].view(shape), buf[2 * n:3 * n].view(shape)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.rope_axes_forward(x, table, pos, sections, out=behind)
+    for tensors, outs in (([x, x], None), ([x, behind], None), ([x, x], [apart, apart]), ([x, apart], [apart, x]),
+                          ([x, apart], [buf[n:2 * n].view(shape), x]), ([apart, x], [x, buf[n:2 * n].view(shape)])):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.rope_axes_forward_many(tensors, table, pos, sections, outs=outs)
+    for kw in ({"out": behind}, {"residual": apart, "out": behind}, {"residual": behind, "out": x}):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.dropout_forward(x, 0.5, seed, **kw)
+    torch.cuda.synchronize()
+    assert bool((buf == 1).all())
+    # neighbours in one allocation, the same input twice, and an input as the output are all right
+    twice = [buf[n:2 * n].view(shape), buf[3 * n:].view(shape)]
+    a, b = ops.rope_axes_forward_many([x, x], table, pos, sections, outs=twice)
+    assert torch.equal(a, b) and bool((x == 1).all())
+    ops.rope_axes_forward_many([x, apart], table, pos, sections)
+    assert torch.equal(x, a) and torch.equal(apart, a)
+    want = ops.dropout_forward(x, 0.5, seed, residual=x)
+    assert torch.equal(ops.dropout_forward(x, 0.5, seed, residual=x, out=x), want)
+    no_error(sa)
