@@ -357,12 +357,19 @@ def _rope_axes_many(tensors, freqs, positions, sections, half: bool, order: str,
     every = tensors + outs + [freqs, positions]
     shapes, dtypes, devices = [t.shape for t in every], [t.dtype for t in every], [t.get_device() for t in every]
     n = len(tensors)
-    key = ("rope_axes", n, tuple(shapes), tuple(dtypes), tuple(devices), tuple(sections), bool(half), order, backward)
     assert positions.is_contiguous(), "positions are a contiguous int32 tensor"
+    sections = tuple(int(s) for s in sections)
+    if torch.compiler.is_compiling():                          # a node of the graph for each tensor
+        kid, sizes = _rope_axes_plan(shapes[:n], shapes[n:-2], dtypes, devices, freqs.shape, positions.shape, sections, bool(half), order, backward)
+        for t, o, (num_bytes, value) in zip(tensors, outs, sizes):
+            if num_bytes:
+                _elementwise(kid, o, None, None, None, t, freqs, None, None, positions, value, 0, 0)
+        return outs
+    key = ("rope_axes", n, tuple(shapes), tuple(dtypes), tuple(devices), sections, bool(half), order, backward)
     plan = _plans.get(key)
     if plan is None:
         plan = _keep_plan(key, _rope_axes_plan(shapes[:n], shapes[n:-2], dtypes, devices, freqs.shape, positions.shape,
-                                               tuple(int(s) for s in sections), bool(half), order, backward))
+                                               sections, bool(half), order, backward))
     kid, sizes = plan
     if sizes[0][0]:                                            # all have elements, or none
         table, where = _aligned(freqs, "freqs"), positions.data_ptr()

@@ -329,3 +329,40 @@ def test_overlapping_arrays_are_refused(sa):
     want = ops.dropout_forward(x, 0.5, seed, residual=x)
     assert torch.equal(ops.dropout_forward(x, 0.5, seed, residual=x, out=x), want)
     no_error(sa)
+
+
+def test_rope_axes_under_torch_compile(sa):
+    from l2_torch_alloc_amd import ops
+    sections = (16, 24, 24)
+    table = ops.freqs_cis_axes_table(sections, 50, 10000.0).cuda()
+    pos = (torch.arange(2 * 7 * 3, dtype=torch.int32) % 50).view(2, 7, 3).cuda()
+    torch.manual_seed(3)
+    q, k = (torch.randn(2, 7, heads, 128, device="cuda", dtype=torch.bfloat16) for heads in (4, 2))
+
+    def rotate(q, k):
+        a, b = ops.rope_axes_forward_many([q * 2, k + 1], table, pos, sections)
+        return a + 1, ops.rope_axes_backward(b, table, pos, sections, out=torch.empty_like(b), half=True, order="turns")
+
+    want = rotate(q, k)
+    for fullgraph in (False, True):
+        compiled = torch.compile(rotate, fullgraph=fullgraph)
+        for _ in range(2):
+            assert all(torch.equal(h, w) for h, w in zip(compiled(q, k), want))
+    no_error(sa)
+
+
+def test_group_norm_under_torch_compile(sa):
+    """Its calls stand between the compiled parts of a function."""
+    from l2_torch_alloc_amd import ops
+    torch.manual_seed(3)
+    x, w, b = torch.randn(2, 30, 64, device="cuda"), torch.randn(64, device="cuda"), torch.randn(64, device="cuda")
+
+    def layer(x):
+        y, stats = ops.group_norm_forward(x * 2, w, b, 8, activation="silu")
+        return ops.group_norm_backward(y + 1, x * 2, w, b, stats, 8, activation="silu")
+
+    want = layer(x)
+    compiled = torch.compile(layer)
+    for _ in range(2):
+        assert all(torch.equal(h, t) for h, t in zip(compiled(x), want))
+    no_error(sa)
