@@ -40,6 +40,7 @@ struct GroupNormPlan {
     long long channel_rows = 0;
     size_t workspace_bytes = 0;
     bool stream = false;            // the arrays do not fit the Infinity Cache together, with a quarter to spare
+    bool merge = false;             // one launch: slabs are no whole memory lines, which the L2 puts together
     long long blocks = 0;           // workgroups of a launch over the array: chunks x slabs x batch_blocks
     int param_blocks = 0;           // workgroups that add up the channels' sums
     bool ok = false;
@@ -55,8 +56,14 @@ constexpr long long kGroupNormMaxLanePixels = 256;         // that a lane adds i
 // A sample's part of the smallest slab that one launch takes: at 20 KiB (2 samples of 256 pixels of 1280 channels) one
 // launch takes 8 us and two take 17, at 80 KiB (2 of 1024 pixels of 640 channels) one takes 15 and two take 11.
 constexpr long long kGroupNormOneLaunchBytes = 32 << 10;
-// Arrays up to this size are read in pieces of rows shorter than a memory line, which costs nothing where few
-// workgroups wait for each other (64 samples of 1024 pixels of 512 channels, 64 MiB: 90 us in such pieces, 38 without).
+// Several times that is still read a second time out of the L2s, if all that run at once hold no more than this (the
+// L2s hold half of it; 16 samples of 1024 pixels of 640 channels, 20 MiB: 15.3 us, two launches 18.2; backward, 40 MiB, 26.6
+// and 29.8; 48 samples, backward, 80 MiB: 86 and 69), every CU has a workgroup and their pieces of a row are half a
+// memory line or more (64 samples of 1024 pixels of 512 channels: pieces of 64 bytes 31.5, of 32 bytes 77, two launches 36.5).
+constexpr long long kGroupNormHeldBytes = 64 << 20;
+constexpr int kGroupNormPieceBytes = 64, kGroupNormLineBytes = 128;
+// Where the arrays exceed the Infinity Cache, pieces are whole lines (256 samples of 256 pixels of 1280 channels: pieces of 80
+// bytes 211 us, two launches 103); arrays up to this size are read in whatever pieces.
 constexpr long long kGroupNormPiecesBytes = 8 << 20;
 // What every workgroup of the second launch may read to add up the chunks' sums by itself: 64 KiB (4 samples of 16384
 // pixels of 128 channels) 20.6 us, 21.7 with a launch between; 256 KiB (65536 pixels of 512 channels) 44.3 and 42.6.
@@ -98,19 +105,29 @@ inline GroupNormPlan plan_group_norm(long long batch, long long pixels, int chan
     if (most_units > most_slice / unit_vectors) most_units = most_slice / unit_vectors > 1 ? most_slice / unit_vectors : 1;
     most_units = (int)gn_ceil(units, gn_ceil(units, most_units));
 
-    // One launch where a sample's part of the smallest slab is little: a workgroup then reads it a second
-    // time out of its caches.  Else the pixels are cut into chunks as well, and a second launch applies
+    // One launch where a sample's part of the smallest slab is little, or the L2s hold the parts of all workgroups that run
+    // at once: they then read it a second time out of the caches.  Else the pixels are cut into chunks as well, and a second launch applies
     // what the first one summed.
-    const long long unit_bytes = pixels * unit_vectors * p.vec * element_bytes;
+    const long long unit_bytes = pixels * unit_vectors * p.vec * element_bytes, piece_bytes = unit_vectors * p.vec * element_bytes;
     // wider slabs while there are workgroups enough without, up to 512 bytes of a row
     int m = 1;
     while (2 * m <= most_units && 2 * m * unit_vectors <= 32 && batch * gn_ceil(units, 2 * m) >= 2 * num_cus &&
            2 * m * unit_bytes <= kGroupNormOneLaunchBytes)
         m *= 2;
-    // (pieces of less than a memory line are all right for little, not for much)
-    const bool pieces = m * unit_vectors * p.vec * element_bytes < 128 && m < units;
-    if (unit_bytes <= kGroupNormOneLaunchBytes && !(pieces && batch * pixels * row_bytes > kGroupNormPiecesBytes)) {
+    p.stream = batch * pixels * row_bytes * (backward ? 3 : 2) > cache_bytes / 4 * 3;
+    bool one = unit_bytes <= kGroupNormOneLaunchBytes &&
+               (m * piece_bytes >= (p.stream ? kGroupNormLineBytes : kGroupNormPieceBytes) || m == units || batch * pixels * row_bytes <= kGroupNormPiecesBytes);
+    if (!one && !p.stream) {
+        m = (int)gn_ceil(kGroupNormPieceBytes, piece_bytes);
+        if (m > units) m = units;
+        const long long all = batch * gn_ceil(units, m), at_once = all < 2 * num_cus ? all : 2 * num_cus;
+        one = m <= most_units && all >= num_cus && at_once * m * unit_bytes * (backward ? 2 : 1) <= kGroupNormHeldBytes;
+        const int slice = m * unit_vectors < most_slice ? m * unit_vectors : most_slice;
+        one = one && gn_ceil(pixels, kGroupNormMaxThreads / slice) <= kGroupNormMaxLanePixels;
+    }
+    if (one) {
         cut(m);
+        p.merge = p.slabs > 1 && (long long)p.slab_vectors * p.vec * element_bytes % kGroupNormLineBytes != 0;
         const long long want = gn_ceil(4ll * num_cus, p.slabs);
         p.batch_blocks = batch < want ? batch : want;
     } else {
@@ -125,13 +142,13 @@ inline GroupNormPlan plan_group_norm(long long batch, long long pixels, int chan
         p.finish = (long long)p.chunks * p.slab_groups * 16 > kGroupNormGatherBytes;
         p.batch_blocks = batch < kGroupNormMaxGrid ? batch : kGroupNormMaxGrid;
     }
-    p.stream = batch * pixels * row_bytes * (backward ? 3 : 2) > cache_bytes / 4 * 3;
     const int lanes = p.slice_vectors * p.rows;
     p.threads = (lanes + 63) / 64 * 64;
     // forward: four doubles a lane.  backward: two floats for each lane and channel, two doubles for each channel
     // of the slice.  Either: two doubles a thread where the chunks' sums are added.
     const size_t slice_channels = (size_t)p.slice_vectors * p.vec;
-    const size_t sums = backward ? p.rows * slice_channels * 2 * sizeof(float) + slice_channels * 2 * sizeof(double) : (size_t)lanes * 4 * sizeof(double);
+    const size_t sums = backward ? p.rows * slice_channels * 2 * sizeof(float) + slice_channels * 2 * sizeof(double) +
+                                   (size_t)(p.rows / p.vec) * slice_channels * 2 * sizeof(double) : (size_t)lanes * 4 * sizeof(double);
     const size_t gather = (size_t)p.threads * 2 * sizeof(double);
     p.lds_bytes = sums > gather ? sums : gather;
     p.blocks = p.batch_blocks * p.slabs * p.chunks;

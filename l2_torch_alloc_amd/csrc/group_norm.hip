@@ -12,7 +12,7 @@
 // write); 8 samples of 64x64 pixels of 320 channels (21 MB) 17 us, 8 and 9 for the two launches, of which about 3 us each
 // go into adding sums up across lanes and workgroups.  Backward with SiLU is bound by the vector ALU too: 21 issue
 // slots a value for the sums, of which an exponential and a reciprocal take eight; 16 samples of 32x32 pixels of 640
-// channels (21 MB) 28 us, 2.2 TB/s.
+// channels (21 MB) 26 us, 2.4 TB/s.
 //
 // A lane keeps one vector of channels and walks pixels, so all accesses of a wave are runs of whole
 // vectors and its sums are per channel, in registers; whatever the number of channels in a group is,
@@ -87,12 +87,15 @@ struct Vec {
 // written back (512x512 pixels of 256 channels: 78 us against 88).  Narrow vectors are left to the L2, which may merge them.
 // The two wait states: hardware reads the data registers of a store wider than 8 bytes for two more issue cycles, and the
 // compiler does not look inside the statement.
-template<bool STREAM, typename W>
+// So are the pieces of memory lines that a workgroup with some of a row's channels writes, where its neighbours on the
+// same XCD write the rest (64 samples of 1024 pixels of 512 channels: 31.6 us, 33.8 written through).
+enum Store { kThrough, kStream, kMerge };
+template<int STORE, typename W>
 __device__ __forceinline__ void store_words(void* to, const W& words) {
-    if constexpr (sizeof(W) == 16) {
-        if constexpr (STREAM) asm volatile("global_store_dwordx4 %0, %1, off sc1 nt\n\ts_nop 1" : : "v"(to), "v"(words) : "memory");
+    if constexpr (sizeof(W) == 16 && STORE != kMerge) {
+        if constexpr (STORE == kStream) asm volatile("global_store_dwordx4 %0, %1, off sc1 nt\n\ts_nop 1" : : "v"(to), "v"(words) : "memory");
         else asm volatile("global_store_dwordx4 %0, %1, off sc1\n\ts_nop 1" : : "v"(to), "v"(words) : "memory");
-    } else if constexpr (STREAM) {
+    } else if constexpr (STORE == kStream) {
         __builtin_nontemporal_store(words, (W*)to);
     } else {
         *(W*)to = words;
@@ -136,12 +139,22 @@ struct Place {
     int tx, ty;
 };
 
-// The grid is (chunks, slabs, samples), so nothing is divided here.
+// The grid is (chunks, slabs, samples).  Workgroups are dealt to the XCDs in turn; those of one launch (NEAR), whose slabs are
+// pieces of rows, are numbered so that each XCD has consecutive ones: a memory line is then fetched into one L2
+// alone (16 samples of 256 pixels of 640 channels: 8.7 us dealt in turn, 7.5 so).
+template<bool NEAR>
 __device__ __forceinline__ Place place_of(const GnArgs& a, int chunk) {
     Place q;
     q.chunk = chunk;
     q.slab = (int)blockIdx.y;
     q.n = blockIdx.z;
+    if constexpr (NEAR) {
+        unsigned int at = blockIdx.z * gridDim.y + blockIdx.y;
+        const unsigned int each = gridDim.y * gridDim.z / 8;
+        if (at < each * 8) at = at % 8 * each + at / 8;
+        q.n = at / gridDim.y;
+        q.slab = (int)(at % gridDim.y);
+    }
     q.first_vector = q.slab * a.slab_vectors;
     q.end_vector = min(q.first_vector + a.slab_vectors, a.row_vectors);
     q.first_group = q.slab * a.slab_groups;
@@ -184,9 +197,9 @@ struct Lane {
     __device__ __forceinline__ V load(const void* array, int run) const {
         return *(const V*)((const char*)array + base + run * step + (run < whole ? off : off_last));
     }
-    template<bool STREAM>
+    template<int STORE>
     __device__ __forceinline__ void store(void* array, int i, const V& value) const {
-        store_words<STREAM>((char*)array + base + i * step + off, value.words);
+        store_words<STORE>((char*)array + base + i * step + off, value.words);
     }
 };
 
@@ -282,8 +295,11 @@ __device__ __forceinline__ void write_part(const GnArgs& a, const Place& q, long
     }
 }
 
-// kApplyStream: as kApply, where the arrays exceed the Infinity Cache.
-enum Mode { kSums, kApply, kApplyStream, kBoth };
+// kApplyStream: as kApply, where the arrays exceed the Infinity Cache.  kBothMerge: as kBoth, where workgroups share
+// memory lines.
+enum Mode { kSums, kApply, kApplyStream, kBoth, kBothMerge };
+constexpr bool does_both(int mode) { return mode == kBoth || mode == kBothMerge; }
+constexpr int store_of(int mode) { return mode == kApplyStream ? kStream : mode == kBothMerge ? kMerge : kThrough; }
 constexpr bool applies_only(int mode) { return mode == kApply || mode == kApplyStream; }
 
 // All workgroups start together and would stay in step: every lane waiting for its batch of loads, then every lane
@@ -521,7 +537,7 @@ __device__ __forceinline__ void load_stats(const float* from, const GnArgs& a, c
     __syncthreads();
 }
 
-template<typename T, int VEC, bool SILU, bool STREAM, int B>
+template<typename T, int VEC, bool SILU, int STORE, int B>
 __device__ __forceinline__ void forward_apply(const GnArgs& a, const Lane<T, VEC>& lane, Vec<T, VEC> (&cur)[B], const float (&mean)[VEC],
                                               const float (&scale)[VEC], const float (&shift)[VEC]) {
     typedef Vec<T, VEC> V;
@@ -542,7 +558,7 @@ __device__ __forceinline__ void forward_apply(const GnArgs& a, const Lane<T, VEC
     for (; i + 2 * B <= lane.whole; i += B) {
         #pragma unroll
         for (int u = 0; u < B; u++) {
-            lane.template store<STREAM>(a.out, i + u, one(cur[u]));
+            lane.template store<STORE>(a.out, i + u, one(cur[u]));
             cur[u] = lane.load(a.x, i + B + u);
             in_order();
         }
@@ -551,7 +567,7 @@ __device__ __forceinline__ void forward_apply(const GnArgs& a, const Lane<T, VEC
     for (; i < lane.runs; i += B) {
         #pragma unroll
         for (int u = 0; u < B; u++) {
-            if (i + u < lane.count) lane.template store<STREAM>(a.out, i + u, one(cur[u]));
+            if (i + u < lane.count) lane.template store<STORE>(a.out, i + u, one(cur[u]));
             if (i + B + u < lane.runs) {
                 cur[u] = lane.load(a.x, i + B + u);
             }
@@ -570,7 +586,7 @@ __global__ __launch_bounds__(kGroupNormMaxThreads, 4) void group_norm_forward(Gn
     extern __shared__ double lds[];
     __shared__ double sums[kGroupNormMaxSlabGroups][2];
     __shared__ float stat[kGroupNormMaxSlabGroups][2];
-    const Place q = place_of(a, (int)blockIdx.x);
+    const Place q = place_of<does_both(MODE)>(a, (int)blockIdx.x);
     long long n = q.n;
     do {
         constexpr int B = forward_batch(MODE);
@@ -599,7 +615,7 @@ __global__ __launch_bounds__(kGroupNormMaxThreads, 4) void group_norm_forward(Gn
                 if (lane.count) {
                     if (!ONE && v0 != q.first_vector) lane.load(pre, a.x, 0);
                     groups_of<VEC>(g, a, q, lane.v);
-                    if constexpr (MODE == kBoth) {
+                    if constexpr (does_both(MODE)) {
                         Vec<T, VEC> cur[B];                       // `pre` stays, to be applied
                         #pragma unroll
                         for (int u = 0; u < B; u++) cur[u] = pre[u];
@@ -639,8 +655,8 @@ __global__ __launch_bounds__(kGroupNormMaxThreads, 4) void group_norm_forward(Gn
                         mean[j] = stat[g[j]][0];
                         scale[j] *= stat[g[j]][1];
                     }
-                    if (a.activation == kGroupNormSilu) forward_apply<T, VEC, true, MODE == kApplyStream, B>(a, lane, pre, mean, scale, shift);
-                    else forward_apply<T, VEC, false, MODE == kApplyStream, B>(a, lane, pre, mean, scale, shift);
+                    if (a.activation == kGroupNormSilu) forward_apply<T, VEC, true, store_of(MODE), B>(a, lane, pre, mean, scale, shift);
+                    else forward_apply<T, VEC, false, store_of(MODE), B>(a, lane, pre, mean, scale, shift);
                 }
                 v0 += a.slice_vectors;
             } while (!ONE && v0 < q.end_vector);
@@ -784,6 +800,7 @@ __device__ __forceinline__ void backward_group_sums(const GnArgs& a, const Place
     const int c0 = v0 * VEC, here = min(v0 + a.slice_vectors, q.end_vector) * VEC - c0;      // channels of the slice
     float* lanes = (float*)lds;                                   // [which][row][channel of the slice]
     double* totals = lds + a.rows * slice_channels;               // [which][channel]
+    double2* partial = (double2*)(totals + 2 * slice_channels);   // [part][channel]
     float* to = a.channel_part + row * 2 * a.channels + c0;
     if (q.ty < a.rows) {
         float* at = lanes + q.ty * slice_channels + q.tx * VEC;
@@ -794,14 +811,39 @@ __device__ __forceinline__ void backward_group_sums(const GnArgs& a, const Place
         }
     }
     __syncthreads();
+    auto add_rows = [&](int c, int first, int step) {
+        double2 t = {0, 0};
+        #pragma unroll 4
+        for (int r = first; r < a.rows; r += step) {
+            t.x += lanes[r * slice_channels + c];
+            t.y += lanes[(a.rows + r) * slice_channels + c];
+        }
+        return t;
+    };
+    // VEC rows of threads are as many as there are channels: each such part adds some of the rows up (8 samples of
+    // 256 pixels of 1280 channels, backward: 14.4 us, 15.9 with one thread to a channel)
+    const int parts = a.rows / VEC;
+    if (parts > 1) {
+        if (q.ty < parts * VEC) {
+            const int c = q.ty % VEC * a.slice_vectors + q.tx, part = q.ty / VEC;
+            partial[part * slice_channels + c] = add_rows(c, part, parts);
+        }
+        __syncthreads();
+    }
     for (int c = (int)threadIdx.x; c < here; c += (int)blockDim.x) {
         float w[1];
         load_params<T, 1>(w, a.weight, a.weight_fp32, c0 + c, 1.0f);
         double t1 = 0, t2 = 0;
-        #pragma unroll 4
-        for (int r = 0; r < a.rows; r++) {
-            t1 += lanes[r * slice_channels + c];
-            t2 += lanes[(a.rows + r) * slice_channels + c];
+        if (parts > 1) {
+            #pragma unroll 4
+            for (int i = 0; i < parts; i++) {
+                t1 += partial[i * slice_channels + c].x;
+                t2 += partial[i * slice_channels + c].y;
+            }
+        } else {
+            const double2 t = add_rows(c, 0, 1);
+            t1 = t.x;
+            t2 = t.y;
         }
         to[c] = add_to_row ? to[c] + (float)t1 : (float)t1;
         to[a.channels + c] = add_to_row ? to[a.channels + c] + (float)t2 : (float)t2;
@@ -840,7 +882,7 @@ __device__ __forceinline__ void backward_group_sums(const GnArgs& a, const Place
 }
 
 // dx = rstd (w dz - c1 - h c2) as dz scale - (x - mean) e - d
-template<typename T, int VEC, bool SILU, bool STREAM, int B>
+template<typename T, int VEC, bool SILU, int STORE, int B>
 __device__ __forceinline__ void backward_apply(const GnArgs& a, const Place& q, long long n, const Lane<T, VEC>& lane,
                                                Vec<T, VEC> (&x)[B], Vec<T, VEC> (&g)[B], float (*stat)[2]) {
     typedef Vec<T, VEC> V;
@@ -873,7 +915,7 @@ __device__ __forceinline__ void backward_apply(const GnArgs& a, const Place& q, 
     for (; i + 2 * B <= lane.whole; i += B) {
         #pragma unroll
         for (int u = 0; u < B; u++) {
-            lane.template store<STREAM>(a.out, i + u, one(x[u], g[u]));
+            lane.template store<STORE>(a.out, i + u, one(x[u], g[u]));
             x[u] = lane.load(a.x, i + B + u);
             g[u] = lane.load(a.dout, i + B + u);
             in_order();
@@ -883,7 +925,7 @@ __device__ __forceinline__ void backward_apply(const GnArgs& a, const Place& q, 
     for (; i < lane.runs; i += B) {
         #pragma unroll
         for (int u = 0; u < B; u++) {
-            if (i + u < lane.count) lane.template store<STREAM>(a.out, i + u, one(x[u], g[u]));
+            if (i + u < lane.count) lane.template store<STORE>(a.out, i + u, one(x[u], g[u]));
             if (i + B + u < lane.runs) {
                 x[u] = lane.load(a.x, i + B + u);
                 g[u] = lane.load(a.dout, i + B + u);
@@ -941,7 +983,7 @@ __global__ __launch_bounds__(kGroupNormMaxThreads, 4) void group_norm_backward(G
         if (block < a.param_blocks) add_params<T>(a, (int)block, lds);
         return;
     }
-    const Place q = place_of(a, (int)blockIdx.x - (applies_only(MODE) ? a.param_x : 0));
+    const Place q = place_of<does_both(MODE)>(a, (int)blockIdx.x - (applies_only(MODE) ? a.param_x : 0));
     const bool silu = a.activation == kGroupNormSilu;
     long long n = q.n;
     do {
@@ -970,7 +1012,7 @@ __global__ __launch_bounds__(kGroupNormMaxThreads, 4) void group_norm_backward(G
                         if (silu) backward_lane_sums<T, VEC, true, B>(a, q, n, lane, x, g, s1, s2);
                         else backward_lane_sums<T, VEC, false, B>(a, q, n, lane, x, g, s1, s2);
                     };
-                    if constexpr (MODE == kBoth) {
+                    if constexpr (does_both(MODE)) {
                         Vec<T, VEC> x[B], g[B];                   // `px` and `pg` stay, to be applied
                         #pragma unroll
                         for (int u = 0; u < B; u++) { x[u] = px[u]; g[u] = pg[u]; }
@@ -1004,8 +1046,8 @@ __global__ __launch_bounds__(kGroupNormMaxThreads, 4) void group_norm_backward(G
                         lane.load(px, a.x, 0);
                         lane.load(pg, a.dout, 0);
                     }
-                    if (silu) backward_apply<T, VEC, true, MODE == kApplyStream, B>(a, q, n, lane, px, pg, stat);
-                    else backward_apply<T, VEC, false, MODE == kApplyStream, B>(a, q, n, lane, px, pg, stat);
+                    if (silu) backward_apply<T, VEC, true, store_of(MODE), B>(a, q, n, lane, px, pg, stat);
+                    else backward_apply<T, VEC, false, store_of(MODE), B>(a, q, n, lane, px, pg, stat);
                 }
                 v0 += a.slice_vectors;
             } while (!ONE && v0 < q.end_vector);
@@ -1061,7 +1103,8 @@ hipError_t forward_of(const GroupNormCall& c, hipStream_t stream) {
     const GnArgs a = args_of(c);
     const dim3 grid = grid_of(p), block((unsigned)p.threads);
     if (p.chunks == 1) {
-        group_norm_forward<T, VEC, kBoth, KIND><<<grid, block, p.lds_bytes, stream>>>(a);
+        if (p.merge) group_norm_forward<T, VEC, kBothMerge, KIND><<<grid, block, p.lds_bytes, stream>>>(a);
+        else group_norm_forward<T, VEC, kBoth, KIND><<<grid, block, p.lds_bytes, stream>>>(a);
         return hipGetLastError();
     }
     group_norm_forward<T, VEC, kSums, KIND><<<grid, block, p.lds_bytes, stream>>>(a);
@@ -1085,7 +1128,8 @@ hipError_t backward_of(const GroupNormCall& c, hipStream_t stream) {
     const dim3 block((unsigned)p.threads);
     const bool params = c.dweight || c.dbias;
     if (p.chunks == 1) {
-        group_norm_backward<T, VEC, kBoth, ONE><<<grid, block, p.lds_bytes, stream>>>(a);
+        if (p.merge) group_norm_backward<T, VEC, kBothMerge, ONE><<<grid, block, p.lds_bytes, stream>>>(a);
+        else group_norm_backward<T, VEC, kBoth, ONE><<<grid, block, p.lds_bytes, stream>>>(a);
         const hipError_t err = hipGetLastError();
         if (err != hipSuccess || !params) return err;
         group_norm_params<T><<<dim3((unsigned)p.param_blocks), dim3(256), 0, stream>>>(a);

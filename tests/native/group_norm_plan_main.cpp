@@ -59,7 +59,9 @@ int main() {
         // doubles for each channel of the slice; two doubles a thread
         const size_t slice_channels = (size_t)p.slice_vectors * p.vec;
         if (backward) REQUIRE(p.lds_bytes >= p.rows * slice_channels * 8 + 2 * slice_channels * 8);
-        else REQUIRE(p.lds_bytes >= (size_t)p.slice_vectors * p.rows * 32);
+        // (and where rows are many, two doubles for each channel and part of the rows)
+        if (backward) REQUIRE(p.lds_bytes >= (p.rows + 2) * slice_channels * 8 + (p.rows / p.vec) * slice_channels * 16);
+        if (!backward) REQUIRE(p.lds_bytes >= (size_t)p.slice_vectors * p.rows * 32);
         REQUIRE(p.lds_bytes >= (size_t)p.threads * 16);
         REQUIRE(p.lds_bytes + kGroupNormMaxSlabGroups * 24 <= 65536);
         // workspace

@@ -349,3 +349,18 @@ def test_overlapping_arrays_are_refused(sa):
     have = ops.group_norm_backward(x, x, w, w, stats, 4, out=x)
     assert all(torch.equal(h, t) for h, t in zip(have, want))
     no_error(sa)
+
+
+@pytest.mark.parametrize("N,P,C,G,dtype", [(16, 900, 640, 32, torch.bfloat16), (16, 700, 640, 32, torch.float32), (128, 700, 66, 3, torch.float16),
+                                           (33, 401, 512, 32, torch.bfloat16), (40, 1024, 640, 32, torch.float16)])
+def test_many_samples_in_pieces_of_rows(sa, N, P, C, G, dtype):
+    """Workgroups that share memory lines: their numbering over the XCDs, and stores that the L2 puts together."""
+    from l2_torch_alloc_amd import ops
+    x, w, b, dout = make(N, P, C, dtype, torch.float32, seed=N + P)
+    xd, wd, bd, gd = x.cuda(), w.cuda(), b.cuda(), dout.cuda()
+    y, stats = ops.group_norm_forward(xd, wd, bd, G, activation="silu")
+    check_forward(y, stats, x, w, b, G, 1e-5, "silu")
+    check_backward(ops.group_norm_backward(gd, xd, wd, bd, stats, G, activation="silu"), dout, x, w, b, stats, G, "silu")
+    again, _ = ops.group_norm_forward(xd, wd, bd, G, activation="silu", out=xd, stats=stats)
+    assert torch.equal(again, y)
+    no_error(sa)

@@ -2,6 +2,7 @@
 workspace and grid), the oracle's gradients against differences, and refusals."""
 import os
 import random
+import re
 import subprocess
 
 import numpy as np
@@ -15,10 +16,17 @@ from l2_torch_alloc_amd import ops, wrapper
 HERE = os.path.dirname(os.path.abspath(__file__))
 
 
-def test_plan(tmp_path):
+def check_plans(tmp_path, text, cases):
     exe = str(tmp_path / "plan")
     subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-fsanitize=address,undefined", os.path.join(HERE, "native", "group_norm_plan_main.cpp"),
                     "-o", exe], check=True, capture_output=True, text=True)
+    proc = subprocess.run([exe], input=text, capture_output=True, text=True, timeout=300)
+    assert proc.returncode == 0 and "ok" in proc.stdout, proc.stdout + proc.stderr
+    assert "cases=%d " % cases in proc.stdout
+    return int(re.search(r"one_launch=(\d+)", proc.stdout)[1])
+
+
+def test_plan(tmp_path):
     rng = random.Random(5)
     cases = [(1, 1, 1, 1), (1, 1, 8192, 1), (1, 7, 8191, 1), (65536, 1, 320, 32), (1, 1 << 20, 512, 32), (2, 64, 1280, 32), (1, 3, 65536, 65536),
              (1, 5, 65536, 1), (16, 1024, 640, 32), (1, 1 << 26, 1, 1), (3, 999, 33, 33), (1 << 20, 1, 8, 2), (1, 262144, 256, 32), (4, 100, 30000, 3)]
@@ -27,9 +35,21 @@ def test_plan(tmp_path):
         channels = groups * rng.choice([1, 1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 33, 40, 64, 129, 1024])
         cases.append((int(2 ** rng.uniform(0, 12)), int(2 ** rng.uniform(0, 20)), channels, groups))
     text = "".join("%d %d %d %d %d %d\n" % (c + (rng.choice([2, 4]), rng.choice([0, 1]))) for c in cases)
-    proc = subprocess.run([exe], input=text, capture_output=True, text=True, timeout=300)
-    assert proc.returncode == 0 and "ok" in proc.stdout, proc.stdout + proc.stderr
-    assert "cases=%d" % len(cases) in proc.stdout
+    check_plans(tmp_path, text, len(cases))
+
+
+def test_plan_of_many_samples(tmp_path):
+    """Where one launch takes pieces of rows that do not fit a workgroup's own caches: vectors of every width, pixels up to
+    what a lane may add."""
+    rng = random.Random(6)
+    cases = []
+    for _ in range(3000):
+        groups = rng.choice([1, 2, 3, 8, 32])
+        channels = groups * rng.choice([1, 2, 3, 8, 10, 20, 33, 40, 65])
+        cases.append((int(2 ** rng.uniform(3, 9)), int(2 ** rng.uniform(5, 13)), channels, groups))
+    cases += [(16, 1024, 640, 32), (256, 3971, 33, 1), (256, 4096, 32, 1), (512, 1985, 33, 1), (128, 700, 66, 3)]
+    text = "".join("%d %d %d %d %d %d\n" % (c + (rng.choice([2, 4]), rng.choice([0, 1]))) for c in cases)
+    assert check_plans(tmp_path, text, len(cases)) > 500
 
 
 @pytest.mark.parametrize("activation", ["none", "silu"])
