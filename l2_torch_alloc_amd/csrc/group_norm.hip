@@ -1145,7 +1145,7 @@ hipError_t backward_of(const GroupNormCall& c, hipStream_t stream) {
     }
     if (params) {
         a.param_blocks = p.param_blocks;
-        a.param_x = (int)gn_ceil(p.param_blocks, (long long)p.slabs * p.batch_blocks);
+        a.param_x = p.param_x;
         grid.x += (unsigned)a.param_x;
     }
     if (p.stream) group_norm_backward<T, VEC, kApplyStream, ONE><<<grid, block, p.lds_bytes, stream>>>(a);

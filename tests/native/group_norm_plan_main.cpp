@@ -38,6 +38,7 @@ int main() {
         REQUIRE(samples >= 1 && samples <= batch && samples <= 65535 && p.slabs <= 65535 && p.blocks == samples * p.slabs * p.chunks);
         const long long others = p.slabs * samples;
         REQUIRE((p.chunks + (p.param_blocks + others - 1) / others) * others <= 0x7fffffffll);
+        REQUIRE((long long)p.param_x * others >= p.param_blocks && (p.chunks + (long long)p.param_x) * others <= 0x7fffffffll);
         // thread numbers are divided by multiplying with 2^20 / slice_vectors
         for (int t = 0; t < p.threads; t++) {
             const unsigned inv = ((1u << 20) + p.slice_vectors - 1) / p.slice_vectors;
