@@ -725,8 +725,8 @@ __device__ __forceinline__ float grad_of_z(float dout, float z) {
 // What a lane needs of its channels to have z and dz of a value: z = (x - mean) scale + shift.
 template<typename T, int VEC>
 struct Channels {
-    float mean[VEC], scale[VEC], shift[VEC];
-    __device__ __forceinline__ void load(const GnArgs& a, const Place& q, long long n, int v, float (&rstd)[VEC]) {
+    float mean[VEC], scale[VEC], shift[VEC], rstd[VEC];
+    __device__ __forceinline__ void load(const GnArgs& a, const Place& q, long long n, int v) {
         int g[VEC];
         load_params<T, VEC>(scale, a.weight, a.weight_fp32, v * VEC, 1.0f);
         load_params<T, VEC>(shift, a.bias, a.weight_fp32, v * VEC, 0.0f);
@@ -744,13 +744,10 @@ struct Channels {
 
 // The sums of dz and of dz h over the lane's pixels, by channel.
 template<typename T, int VEC, bool SILU, int B>
-__device__ __forceinline__ void backward_lane_sums(const GnArgs& a, const Place& q, long long n, const Lane<T, VEC>& lane,
+__device__ __forceinline__ void backward_lane_sums(const GnArgs& a, const Lane<T, VEC>& lane, const Channels<T, VEC>& ch,
                                                    Vec<T, VEC> (&x)[B], Vec<T, VEC> (&g)[B],
                                                    float (&s1)[VEC], float (&s2)[VEC]) {
     typedef Vec<T, VEC> V;
-    Channels<T, VEC> ch;
-    float rstd[VEC];
-    ch.load(a, q, n, lane.v, rstd);
     #pragma unroll
     for (int j = 0; j < VEC; j++) s1[j] = s2[j] = 0;
     auto add = [&](const V& in, const V& grad) {
@@ -788,14 +785,14 @@ __device__ __forceinline__ void backward_lane_sums(const GnArgs& a, const Place&
         }
     }
     #pragma unroll
-    for (int j = 0; j < VEC; j++) s2[j] *= rstd[j];
+    for (int j = 0; j < VEC; j++) s2[j] *= ch.rstd[j];
 }
 
 // Adds the lanes' sums up to channels (for the gradients of weight and bias, into `row` of the workspace) and
 // those, weighted, to the slab's groups.
 template<typename T, int VEC, int MODE, bool ONE>
 __device__ __forceinline__ void backward_group_sums(const GnArgs& a, const Place& q, long long n, int v0, bool on, const float (&s1)[VEC], const float (&s2)[VEC],
-                                                    double* lds, double (*sums)[2], float (*stat)[2], long long row, bool add_to_row) {
+                                                    float weight, double* lds, double (*sums)[2], float (*stat)[2], long long row, bool add_to_row) {
     const int slice_channels = a.slice_vectors * VEC;
     const int c0 = v0 * VEC, here = min(v0 + a.slice_vectors, q.end_vector) * VEC - c0;      // channels of the slice
     float* lanes = (float*)lds;                                   // [which][row][channel of the slice]
@@ -831,8 +828,8 @@ __device__ __forceinline__ void backward_group_sums(const GnArgs& a, const Place
         __syncthreads();
     }
     for (int c = (int)threadIdx.x; c < here; c += (int)blockDim.x) {
-        float w[1];
-        load_params<T, 1>(w, a.weight, a.weight_fp32, c0 + c, 1.0f);
+        float w[1] = {weight};
+        if (!ONE || c != (int)threadIdx.x) load_params<T, 1>(w, a.weight, a.weight_fp32, c0 + c, 1.0f);
         double t1 = 0, t2 = 0;
         if (parts > 1) {
             #pragma unroll 4
@@ -883,18 +880,16 @@ __device__ __forceinline__ void backward_group_sums(const GnArgs& a, const Place
 
 // dx = rstd (w dz - c1 - h c2) as dz scale - (x - mean) e - d
 template<typename T, int VEC, bool SILU, int STORE, int B>
-__device__ __forceinline__ void backward_apply(const GnArgs& a, const Place& q, long long n, const Lane<T, VEC>& lane,
+__device__ __forceinline__ void backward_apply(const GnArgs& a, const Place& q, const Lane<T, VEC>& lane, const Channels<T, VEC>& ch,
                                                Vec<T, VEC> (&x)[B], Vec<T, VEC> (&g)[B], float (*stat)[2]) {
     typedef Vec<T, VEC> V;
-    Channels<T, VEC> ch;
     float d[VEC], e[VEC];
     int gr[VEC];
-    ch.load(a, q, n, lane.v, d);
     groups_of<VEC>(gr, a, q, lane.v);
     #pragma unroll
     for (int j = 0; j < VEC; j++) {
-        e[j] = d[j] * d[j] * stat[gr[j]][1];
-        d[j] *= stat[gr[j]][0];
+        e[j] = ch.rstd[j] * ch.rstd[j] * stat[gr[j]][1];
+        d[j] = ch.rstd[j] * stat[gr[j]][0];
     }
     auto one = [&](const V& in, const V& grad) {
         float xs[VEC], gs[VEC];
@@ -988,17 +983,26 @@ __global__ __launch_bounds__(kGroupNormMaxThreads, 4) void group_norm_backward(G
     long long n = q.n;
     do {
         constexpr int B = backward_batch(MODE);
+        constexpr bool KEEP = ONE && does_both(MODE);             // what a lane needs of its channels, from the sums on
         Vec<T, VEC> px[B], pg[B];
+        Channels<T, VEC> ch;
+        float weight[1] = {1.0f};                                 // of the channel that this thread adds up
         const bool kept = ONE || applies_only(MODE) || q.end_vector - q.first_vector <= a.slice_vectors;
         {
             const Lane<T, VEC> lane(a, q, n, q.first_vector);
             if (lane.count) {
                 lane.load(px, a.x, 0);
                 lane.load(pg, a.dout, 0);
+                if constexpr (KEEP) ch.load(a, q, n, lane.v);
             }
         }
         if constexpr (!applies_only(MODE)) {
-            if constexpr (!ONE) clear_sums(q, sums);
+            if constexpr (ONE) {
+                const int c = q.first_vector * VEC + (int)threadIdx.x;
+                if (c < a.channels) load_params<T, 1>(weight, a.weight, a.weight_fp32, c, 1.0f);
+            } else {
+                clear_sums(q, sums);
+            }
             int v0 = q.first_vector;
             do {
                 const Lane<T, VEC> lane(a, q, n, v0);
@@ -1008,9 +1012,10 @@ __global__ __launch_bounds__(kGroupNormMaxThreads, 4) void group_norm_backward(G
                         lane.load(px, a.x, 0);
                         lane.load(pg, a.dout, 0);
                     }
+                    if constexpr (!KEEP) ch.load(a, q, n, lane.v);
                     auto sum = [&](Vec<T, VEC> (&x)[B], Vec<T, VEC> (&g)[B]) {
-                        if (silu) backward_lane_sums<T, VEC, true, B>(a, q, n, lane, x, g, s1, s2);
-                        else backward_lane_sums<T, VEC, false, B>(a, q, n, lane, x, g, s1, s2);
+                        if (silu) backward_lane_sums<T, VEC, true, B>(a, lane, ch, x, g, s1, s2);
+                        else backward_lane_sums<T, VEC, false, B>(a, lane, ch, x, g, s1, s2);
                     };
                     if constexpr (does_both(MODE)) {
                         Vec<T, VEC> x[B], g[B];                   // `px` and `pg` stay, to be applied
@@ -1021,7 +1026,7 @@ __global__ __launch_bounds__(kGroupNormMaxThreads, 4) void group_norm_backward(G
                         sum(px, pg);
                     }
                 }
-                backward_group_sums<T, VEC, MODE, ONE>(a, q, n, v0, lane.count != 0, s1, s2, lds, sums, stat, q.n * a.chunks + q.chunk, n != q.n);
+                backward_group_sums<T, VEC, MODE, ONE>(a, q, n, v0, lane.count != 0, s1, s2, weight[0], lds, sums, stat, q.n * a.chunks + q.chunk, n != q.n);
                 v0 += a.slice_vectors;
             } while (!ONE && v0 < q.end_vector);
         }
@@ -1046,8 +1051,9 @@ __global__ __launch_bounds__(kGroupNormMaxThreads, 4) void group_norm_backward(G
                         lane.load(px, a.x, 0);
                         lane.load(pg, a.dout, 0);
                     }
-                    if (silu) backward_apply<T, VEC, true, store_of(MODE), B>(a, q, n, lane, px, pg, stat);
-                    else backward_apply<T, VEC, false, store_of(MODE), B>(a, q, n, lane, px, pg, stat);
+                    if constexpr (!KEEP) ch.load(a, q, n, lane.v);
+                    if (silu) backward_apply<T, VEC, true, store_of(MODE), B>(a, q, lane, ch, px, pg, stat);
+                    else backward_apply<T, VEC, false, store_of(MODE), B>(a, q, lane, ch, px, pg, stat);
                 }
                 v0 += a.slice_vectors;
             } while (!ONE && v0 < q.end_vector);
