@@ -310,19 +310,16 @@ def _keep_plan(key: Tuple, plan: Tuple) -> Tuple:
     return plan
 
 
+# Workgroups finish in any order: an output may be an input itself, element for element, but no part of another array.
+_OVERLAP = "an output overlaps another array of the call"
+
+
 def _aligned(t: torch.Tensor, name: str) -> int:
     """Address of a tensor whose device is known: contiguous and 16-byte aligned."""
     assert t.is_contiguous(), name + " must be contiguous"
     ptr = t.data_ptr()
     assert not ptr & 15, name + " must be 16-byte aligned"
     return ptr
-
-
-def _refuse_overlap(out: int, out_bytes: int, array: int, array_bytes: int) -> None:
-    """Of an output and another array of a launch, by address: workgroups finish in any order, so an output may
-    be an input itself, element for element, but not share part of another array's memory."""
-    if out < array + array_bytes and array < out + out_bytes:
-        raise ValueError("an output overlaps another array of the call")
 
 
 def _rope_axes_plan(shapes, out_shapes, dtypes, devices, freqs_shape, positions_shape, sections, half, order, backward):
@@ -346,7 +343,7 @@ def _rope_axes_plan(shapes, out_shapes, dtypes, devices, freqs_shape, positions_
         assert o == t, "an output is like its tensor"
     assert all(d == dtypes[0] for d in dtypes[:-2]), "tensors and outputs share one type"
     assert devices[0] >= 0 and all(d == devices[0] for d in devices), "tensors, outputs, table and positions live on one GPU"
-    kid = _kernel("rope_axes", (head_dim, sections, dtype, half, order, backward))
+    kid = _kernel("rope_axes", (head_dim, tuple(int(s) for s in sections), dtype, half, order, backward))
     size = 4 if dtype == "fp32" else 2
     return kid, [(t.numel() * size, headers.rope_axes_sideband(t[2], freqs_shape[0])) for t in shapes]
 
@@ -358,7 +355,7 @@ def _rope_axes_many(tensors, freqs, positions, sections, half: bool, order: str,
     shapes, dtypes, devices = [t.shape for t in every], [t.dtype for t in every], [t.get_device() for t in every]
     n = len(tensors)
     assert positions.is_contiguous(), "positions are a contiguous int32 tensor"
-    sections = tuple(int(s) for s in sections)
+    sections = tuple(sections)
     if torch.compiler.is_compiling():                          # a node of the graph for each tensor
         kid, sizes = _rope_axes_plan(shapes[:n], shapes[n:-2], dtypes, devices, freqs.shape, positions.shape, sections, bool(half), order, backward)
         for t, o, (num_bytes, value) in zip(tensors, outs, sizes):
@@ -375,13 +372,11 @@ def _rope_axes_many(tensors, freqs, positions, sections, half: bool, order: str,
         table, where = _aligned(freqs, "freqs"), positions.data_ptr()
         arrays = [(_aligned(o, "out"), _aligned(t, "x"), size) for t, o, (size, _) in zip(tensors, outs, sizes)]
         for i, (out, inp, size) in enumerate(arrays):
-            if out != inp:
-                _refuse_overlap(out, size, inp, size)
-            for other_out, other_inp, other_size in arrays[:i]:
-                _refuse_overlap(out, size, other_out, other_size)
-                _refuse_overlap(out, size, other_inp, other_size)
-                if out != inp:
-                    _refuse_overlap(other_out, other_size, inp, size)
+            end, overlap = out + size, out != inp and out < inp + size and inp < out + size
+            for o, x, n_bytes in arrays[:i]:
+                overlap = overlap or out < o + n_bytes and o < end or out < x + n_bytes and x < end or o < inp + size and inp < o + n_bytes
+            if overlap:
+                raise ValueError(_OVERLAP)
         packed = b"".join([_SEGMENT.pack(size, out, 0, 0, 0, inp, table, 0, 0, where, value)
                            for (out, inp, size), (_, value) in zip(arrays, sizes)])
         device, stream = wrapper._device_and_stream(freqs)
@@ -446,10 +441,8 @@ def _dropout(x: torch.Tensor, p: float, seed: torch.Tensor, residual: Optional[t
             kid = _kernel("dropout", (dtype, residual is not None))
             size, to, first = x.numel() * x.element_size(), _aligned(out, "out"), _aligned(x, "x")
             second = 0 if residual is None else _aligned(residual, "residual")
-            if to != first:
-                _refuse_overlap(to, size, first, size)
-            if second and to != second:
-                _refuse_overlap(to, size, second, size)
+            if 0 < abs(to - first) < size or second and 0 < abs(to - second) < size:
+                raise ValueError(_OVERLAP)
             device, stream = wrapper._device_and_stream(x)
             wrapper.library().sideaware_elementwise(kid, size, to, 0, 0, 0, first, second, 0, 0, seed.data_ptr(), threshold, 0, 0, device, stream)
     return out
