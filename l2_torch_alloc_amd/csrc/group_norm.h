@@ -69,13 +69,14 @@ constexpr long long kGroupNormPiecesBytes = 8 << 20;
 // What every workgroup of the second launch may read to add up the chunks' sums by itself: 64 KiB (4 samples of 16384
 // pixels of 128 channels) 20.6 us, 21.7 with a launch between; 256 KiB (65536 pixels of 512 channels) 44.3 and 42.6.
 constexpr long long kGroupNormGatherBytes = 64 << 10;
+constexpr long long kGroupNormCacheBytes = 256ll << 20;    // the Infinity Cache
 constexpr long long kGroupNormMaxGrid = 65535;            // of the second and third axis
 constexpr long long kGroupNormMaxRowsBytes = 1ll << 30;    // a lane's offset among the rows has 32 bits
 
 inline long long gn_ceil(long long a, long long b) { return (a + b - 1) / b; }
 
 inline GroupNormPlan plan_group_norm(long long batch, long long pixels, int channels, int groups, int element_bytes, bool backward,
-                                     int num_cus, long long cache_bytes = 256ll << 20) {
+                                     int num_cus, long long cache_bytes = kGroupNormCacheBytes) {
     GroupNormPlan p;
     if (batch < 1 || pixels < 1 || channels < 1 || groups < 1 || channels % groups || num_cus < 1) return p;
     p.vec = 16 / element_bytes;
@@ -115,10 +116,13 @@ inline GroupNormPlan plan_group_norm(long long batch, long long pixels, int chan
     while (2 * m <= most_units && 2 * m * unit_vectors <= 32 && batch * gn_ceil(units, 2 * m) >= 2 * num_cus &&
            2 * m * unit_bytes <= kGroupNormOneLaunchBytes)
         m *= 2;
-    p.stream = batch * pixels * row_bytes * (backward ? 3 : 2) > cache_bytes / 4 * 3;
+    const long long array_bytes = batch * pixels * row_bytes, all_bytes = array_bytes * (backward ? 3 : 2);
+    // (how the work is cut, and with it the workspace, does not depend on what a user tunes)
+    const bool beyond = all_bytes > kGroupNormCacheBytes / 4 * 3;
+    p.stream = all_bytes > cache_bytes / 4 * 3;
     bool one = unit_bytes <= kGroupNormOneLaunchBytes &&
-               (m * piece_bytes >= (p.stream ? kGroupNormLineBytes : kGroupNormPieceBytes) || m == units || batch * pixels * row_bytes <= kGroupNormPiecesBytes);
-    if (!one && !p.stream) {
+               (m * piece_bytes >= (beyond ? kGroupNormLineBytes : kGroupNormPieceBytes) || m == units || array_bytes <= kGroupNormPiecesBytes);
+    if (!one && !beyond) {
         m = (int)gn_ceil(kGroupNormPieceBytes, piece_bytes);
         if (m > units) m = units;
         const long long all = batch * gn_ceil(units, m), at_once = all < 2 * num_cus ? all : 2 * num_cus;

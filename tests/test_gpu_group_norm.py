@@ -364,3 +364,21 @@ def test_many_samples_in_pieces_of_rows(sa, N, P, C, G, dtype):
     again, _ = ops.group_norm_forward(xd, wd, bd, G, activation="silu", out=xd, stats=stats)
     assert torch.equal(again, y)
     no_error(sa)
+
+
+def test_workspace_does_not_depend_on_tuning(sa):
+    from l2_torch_alloc_amd import ops
+    lib = sa.library()
+    x, w, b, dout = (t.cuda() for t in make(16, 900, 640, torch.bfloat16, torch.float32))
+    want, stats = ops.group_norm_forward(x, w, b, 32, activation="silu")
+    grads = ops.group_norm_backward(dout, x, w, b, stats, 32, activation="silu")
+    before = lib.sideaware_tune_get(b"cache_bytes")
+    try:
+        for cache in (1 << 16, 1 << 40):
+            assert lib.sideaware_tune(b"cache_bytes", cache) == 0
+            assert torch.equal(ops.group_norm_forward(x, w, b, 32, activation="silu")[0], want)
+            got = ops.group_norm_backward(dout, x, w, b, stats, 32, activation="silu")
+            assert all(torch.equal(g, t) for g, t in zip(got, grads))
+    finally:
+        lib.sideaware_tune(b"cache_bytes", before)
+    no_error(sa)
