@@ -75,6 +75,21 @@ constexpr long long kGroupNormMaxRowsBytes = 1ll << 30;    // a lane's offset am
 
 inline long long gn_ceil(long long a, long long b) { return (a + b - 1) / b; }
 
+// The most groups that one vector's channels belong to.  Vectors start d, 2d, ... channels into a group, d being the
+// greatest common divisor of the two lengths; one that starts at a group's last d has the most, those d channels and
+// vec - d more: 3 for a vector of 8 and groups of 5 (1 + 5 + 2 channels), 1 where groups are whole vectors.
+constexpr int gn_groups_of_vector(int vec, int group_channels) {
+    int d = vec, rest = group_channels;
+    while (rest) {
+        const int next = d % rest;
+        d = rest;
+        rest = next;
+    }
+    return 1 + (vec - d + group_channels - 1) / group_channels;
+}
+// How often the lanes' sums go through LDS, two groups of every vector at a time.
+constexpr int gn_sum_passes(int vec, int group_channels) { return (gn_groups_of_vector(vec, group_channels) + 1) / 2; }
+
 inline GroupNormPlan plan_group_norm(long long batch, long long pixels, int channels, int groups, int element_bytes, bool backward,
                                      int num_cus, long long cache_bytes = kGroupNormCacheBytes) {
     GroupNormPlan p;

@@ -359,13 +359,13 @@ __device__ __forceinline__ void forward_lane_sums(const GnArgs& a, const Lane<T,
     }
 }
 
-// Adds the lanes' sums up to the slab's groups.  A vector of channels touches one or two groups, or, where
-// groups are narrower than it, up to VEC of them, which go through LDS two at a time: each lane leaves its
-// two groups' sums there, and the threads of a group pick up those of the vectors it has a part in.
+// Adds the lanes' sums up to the slab's groups.  A vector of channels touches one or two groups, or, where groups are
+// narrower than it, up to VEC of them (gn_groups_of_vector), which go through LDS two at a time: each lane leaves its two
+// groups' sums there, and the threads of a group pick up those of the vectors it has a part in.
 template<int VEC>
 __device__ __forceinline__ void forward_group_sums(const GnArgs& a, const Place& q, int v0, int count, const int (&g)[VEC], const float (&pivot)[VEC],
                                                    const float (&s1)[VEC], const float (&s2)[VEC], double* lds, double (*sums)[2]) {
-    const int passes = a.group_channels >= VEC ? 1 : (VEC / a.group_channels + 2) / 2;
+    const int passes = gn_sum_passes(VEC, a.group_channels);
     const int end = min(v0 + a.slice_vectors, q.end_vector) - q.first_vector, start = v0 - q.first_vector;   // vectors of the slab
     const int per = 1 << a.per_group_log2;
     const int first = (int)threadIdx.x >> a.per_group_log2, part = (int)threadIdx.x & (per - 1), step = (int)blockDim.x >> a.per_group_log2;
@@ -403,7 +403,7 @@ __device__ __forceinline__ void forward_group_sums(const GnArgs& a, const Place&
                 const int c0 = at * a.group_channels;
                 const int lo = max(c0 / VEC, start), hi = min((c0 + a.group_channels - 1) / VEC + 1, end);
                 for (int w = lo; w < hi; w++) {
-                    // which of its vector's groups this one is
+                    // which of its vector's groups this one is (with one pass a vector has two at most)
                     int slot = w * VEC < c0 ? 1 : 0;
                     if (passes > 1) slot = at - group_of(a, w * VEC) - 2 * pass;
                     if (slot == 0 || slot == 1) {
