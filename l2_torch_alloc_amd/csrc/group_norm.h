@@ -89,6 +89,9 @@ constexpr int gn_groups_of_vector(int vec, int group_channels) {
 }
 // How often the lanes' sums go through LDS, two groups of every vector at a time.
 constexpr int gn_sum_passes(int vec, int group_channels) { return (gn_groups_of_vector(vec, group_channels) + 1) / 2; }
+// Backward, where in LDS the pairs of doubles of the parts of the rows lie, in doubles: behind two floats for each lane's
+// channel and two doubles for each channel of the slice, on a pair's boundary (7 channels, 73 rows: 525 doubles come first).
+constexpr int gn_pairs_at(int rows, int slice_channels) { return ((rows + 2) * slice_channels + 1) / 2 * 2; }
 
 inline GroupNormPlan plan_group_norm(long long batch, long long pixels, int channels, int groups, int element_bytes, bool backward,
                                      int num_cus, long long cache_bytes = kGroupNormCacheBytes) {
@@ -165,10 +168,11 @@ inline GroupNormPlan plan_group_norm(long long batch, long long pixels, int chan
     const int lanes = p.slice_vectors * p.rows;
     p.threads = (lanes + 63) / 64 * 64;
     // forward: four doubles a lane.  backward: two floats for each lane and channel, two doubles for each channel
-    // of the slice.  Either: two doubles a thread where the chunks' sums are added.
-    const size_t slice_channels = (size_t)p.slice_vectors * p.vec;
-    const size_t sums = backward ? p.rows * slice_channels * 2 * sizeof(float) + slice_channels * 2 * sizeof(double) +
-                                   (size_t)(p.rows / p.vec) * slice_channels * 2 * sizeof(double) : (size_t)lanes * 4 * sizeof(double);
+    // of the slice, then two doubles for each part of the rows and channel.  Either: two doubles a thread where the chunks'
+    // sums are added.
+    const int slice_channels = p.slice_vectors * p.vec;
+    const size_t sums = backward ? gn_pairs_at(p.rows, slice_channels) * sizeof(double) + (size_t)(p.rows / p.vec) * slice_channels * 2 * sizeof(double)
+                                 : (size_t)lanes * 4 * sizeof(double);
     const size_t gather = (size_t)p.threads * 2 * sizeof(double);
     p.lds_bytes = sums > gather ? sums : gather;
     p.blocks = p.batch_blocks * p.slabs * p.chunks;

@@ -583,9 +583,9 @@ enum Kind { kLoops, kOne, kOneWide };
 template<typename T, int VEC, int MODE, int KIND>
 __global__ __launch_bounds__(kGroupNormMaxThreads, 4) void group_norm_forward(GnArgs a) {
     constexpr bool ONE = KIND != kLoops, AT_ONCE = KIND == kOneWide;
-    extern __shared__ double lds[];
+    extern __shared__ __attribute__((aligned(16))) double lds[];
     __shared__ double sums[kGroupNormMaxSlabGroups][2];
-    __shared__ float stat[kGroupNormMaxSlabGroups][2];
+    __shared__ __attribute__((aligned(8))) float stat[kGroupNormMaxSlabGroups][2];
     const Place q = place_of<does_both(MODE)>(a, (int)blockIdx.x);
     long long n = q.n;
     do {
@@ -797,7 +797,7 @@ __device__ __forceinline__ void backward_group_sums(const GnArgs& a, const Place
     const int c0 = v0 * VEC, here = min(v0 + a.slice_vectors, q.end_vector) * VEC - c0;      // channels of the slice
     float* lanes = (float*)lds;                                   // [which][row][channel of the slice]
     double* totals = lds + a.rows * slice_channels;               // [which][channel]
-    double2* partial = (double2*)(totals + 2 * slice_channels);   // [part][channel]
+    double2* partial = (double2*)(lds + gn_pairs_at(a.rows, slice_channels));                // [part][channel]
     float* to = a.channel_part + row * 2 * a.channels + c0;
     if (q.ty < a.rows) {
         float* at = lanes + q.ty * slice_channels + q.tx * VEC;
@@ -970,9 +970,9 @@ __device__ __forceinline__ void add_params(const GnArgs& a, int block, double* l
 
 template<typename T, int VEC, int MODE, bool ONE>
 __global__ __launch_bounds__(kGroupNormMaxThreads, 4) void group_norm_backward(GnArgs a) {
-    extern __shared__ double lds[];
+    extern __shared__ __attribute__((aligned(16))) double lds[];
     __shared__ double sums[kGroupNormMaxSlabGroups][2];
-    __shared__ float stat[kGroupNormMaxSlabGroups][2];
+    __shared__ __attribute__((aligned(8))) float stat[kGroupNormMaxSlabGroups][2];
     if (applies_only(MODE) && (int)blockIdx.x < a.param_x) {          // a part of the grid that comes first
         const long long block = ((long long)blockIdx.z * gridDim.y + blockIdx.y) * a.param_x + blockIdx.x;
         if (block < a.param_blocks) add_params<T>(a, (int)block, lds);
@@ -1065,7 +1065,7 @@ __global__ __launch_bounds__(kGroupNormMaxThreads, 4) void group_norm_backward(G
 
 template<typename T>
 __global__ __launch_bounds__(256) void group_norm_params(GnArgs a) {
-    __shared__ double lds[256 * 2];
+    __shared__ __attribute__((aligned(16))) double lds[256 * 2];
     add_params<T>(a, blockIdx.x, lds);
 }
 
