@@ -154,8 +154,10 @@ class _Segment(ctypes.Structure):
                 ("sideband_memory", ctypes.c_void_p), ("sideband_value", ctypes.c_int)]
 
 
-# The same layout, filled in one step (field by field costs a small launch several times its C call).
-_SEGMENT = struct.Struct("=Q4Q4QQi4x")
+# The same layout, filled in one step (field by field costs a small launch several times its C call).  The sideband value
+# goes in as the word its low 32 bits are, as ctypes passes it in a single launch: a bit pattern of 2^31 or more is one too.
+_SEGMENT = struct.Struct("=Q4Q4QQI4x")
+_WORD = 0xFFFFFFFF
 assert _SEGMENT.size == ctypes.sizeof(_Segment)
 
 
@@ -172,7 +174,7 @@ def elementwise_batch(kernel_id: int, segments) -> None:
         for i, t in enumerate(ins):
             inp[i] = wrapper._check(t, "in%d" % i)
             first = t if first is None else first
-        packed.append(_SEGMENT.pack(num_bytes, *out, *inp, sideband.data_ptr() if sideband is not None else 0, int(value)))
+        packed.append(_SEGMENT.pack(num_bytes, *out, *inp, sideband.data_ptr() if sideband is not None else 0, int(value) & _WORD))
     device, stream = wrapper._device_and_stream(first)      # where the arrays live, the current device or not
     wrapper.library().sideaware_elementwise_batch(kernel_id, len(packed), b"".join(packed), device, stream)
 
@@ -377,7 +379,7 @@ def _rope_axes_many(tensors, freqs, positions, sections, half: bool, order: str,
                 overlap = overlap or out < o + n_bytes and o < end or out < x + n_bytes and x < end or o < inp + size and inp < o + n_bytes
             if overlap:
                 raise ValueError(_OVERLAP)
-        packed = b"".join([_SEGMENT.pack(size, out, 0, 0, 0, inp, table, 0, 0, where, value)
+        packed = b"".join([_SEGMENT.pack(size, out, 0, 0, 0, inp, table, 0, 0, where, value & _WORD)
                            for (out, inp, size), (_, value) in zip(arrays, sizes)])
         device, stream = wrapper._device_and_stream(freqs)
         wrapper.library().sideaware_elementwise_batch(kid, n, packed, device, stream)
