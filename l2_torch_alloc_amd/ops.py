@@ -325,7 +325,7 @@ def _aligned(t: torch.Tensor, name: str) -> int:
 
 
 def _rope_axes_plan(shapes, out_shapes, dtypes, devices, freqs_shape, positions_shape, sections, half, order, backward):
-    """The kernel and, for each tensor with elements, its bytes and sideband value."""
+    """The kernel, for each tensor its bytes and sideband value, and the bytes of the table and the positions."""
     first = shapes[0]
     assert len(first) == 4, "activations are (B, T, heads, head_dim)"
     B, T, _, head_dim = first
@@ -347,7 +347,8 @@ def _rope_axes_plan(shapes, out_shapes, dtypes, devices, freqs_shape, positions_
     assert devices[0] >= 0 and all(d == devices[0] for d in devices), "tensors, outputs, table and positions live on one GPU"
     kid = _kernel("rope_axes", (head_dim, tuple(int(s) for s in sections), dtype, half, order, backward))
     size = 4 if dtype == "fp32" else 2
-    return kid, [(t.numel() * size, headers.rope_axes_sideband(t[2], freqs_shape[0])) for t in shapes]
+    sizes = [(t.numel() * size, headers.rope_axes_sideband(t[2], freqs_shape[0])) for t in shapes]
+    return kid, sizes, freqs_shape[0] * freqs_shape[1] * 4, B * T * len(sections) * 4
 
 
 def _rope_axes_many(tensors, freqs, positions, sections, half: bool, order: str, backward: bool, outs):
@@ -359,7 +360,7 @@ def _rope_axes_many(tensors, freqs, positions, sections, half: bool, order: str,
     assert positions.is_contiguous(), "positions are a contiguous int32 tensor"
     sections = tuple(sections)
     if torch.compiler.is_compiling():                          # a node of the graph for each tensor
-        kid, sizes = _rope_axes_plan(shapes[:n], shapes[n:-2], dtypes, devices, freqs.shape, positions.shape, sections, bool(half), order, backward)
+        kid, sizes, _, _ = _rope_axes_plan(shapes[:n], shapes[n:-2], dtypes, devices, freqs.shape, positions.shape, sections, bool(half), order, backward)
         for t, o, (num_bytes, value) in zip(tensors, outs, sizes):
             if num_bytes:
                 _elementwise(kid, o, None, None, None, t, freqs, None, None, positions, value, 0, 0)
@@ -369,12 +370,14 @@ def _rope_axes_many(tensors, freqs, positions, sections, half: bool, order: str,
     if plan is None:
         plan = _keep_plan(key, _rope_axes_plan(shapes[:n], shapes[n:-2], dtypes, devices, freqs.shape, positions.shape,
                                                sections, bool(half), order, backward))
-    kid, sizes = plan
+    kid, sizes, table_bytes, where_bytes = plan
     if sizes[0][0]:                                            # all have elements, or none
         table, where = _aligned(freqs, "freqs"), positions.data_ptr()
         arrays = [(_aligned(o, "out"), _aligned(t, "x"), size) for t, o, (size, _) in zip(tensors, outs, sizes)]
         for i, (out, inp, size) in enumerate(arrays):
-            end, overlap = out + size, out != inp and out < inp + size and inp < out + size
+            end = out + size
+            overlap = (out != inp and out < inp + size and inp < end or out < table + table_bytes and table < end
+                       or out < where + where_bytes and where < end)
             for o, x, n_bytes in arrays[:i]:
                 overlap = overlap or out < o + n_bytes and o < end or out < x + n_bytes and x < end or o < inp + size and inp < o + n_bytes
             if overlap:
@@ -443,10 +446,11 @@ def _dropout(x: torch.Tensor, p: float, seed: torch.Tensor, residual: Optional[t
             kid = _kernel("dropout", (dtype, residual is not None))
             size, to, first = x.numel() * x.element_size(), _aligned(out, "out"), _aligned(x, "x")
             second = 0 if residual is None else _aligned(residual, "residual")
-            if 0 < abs(to - first) < size or second and 0 < abs(to - second) < size:
+            state = seed.data_ptr()
+            if 0 < abs(to - first) < size or second and 0 < abs(to - second) < size or to < state + 16 and state < to + size:
                 raise ValueError(_OVERLAP)
             device, stream = wrapper._device_and_stream(x)
-            wrapper.library().sideaware_elementwise(kid, size, to, 0, 0, 0, first, second, 0, 0, seed.data_ptr(), threshold, 0, 0, device, stream)
+            wrapper.library().sideaware_elementwise(kid, size, to, 0, 0, 0, first, second, 0, 0, state, threshold, 0, 0, device, stream)
     return out
 
 
