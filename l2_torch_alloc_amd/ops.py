@@ -354,17 +354,19 @@ def _rope_axes_plan(shapes, out_shapes, dtypes, devices, freqs_shape, positions_
 def _rope_axes_many(tensors, freqs, positions, sections, half: bool, order: str, backward: bool, outs):
     tensors = list(tensors)
     outs = tensors if outs is None else list(outs)
+    if torch.compiler.is_compiling():
+        torch.ops.sideaware.rope_axes(tensors, freqs, positions, [int(s) for s in sections], bool(half), order, backward, outs)
+    else:
+        _rope_axes_launch(tensors, freqs, positions, sections, half, order, backward, outs)
+    return outs
+
+
+def _rope_axes_launch(tensors, freqs, positions, sections, half: bool, order: str, backward: bool, outs) -> None:
     every = tensors + outs + [freqs, positions]
     shapes, dtypes, devices = [t.shape for t in every], [t.dtype for t in every], [t.get_device() for t in every]
     n = len(tensors)
     assert positions.is_contiguous(), "positions are a contiguous int32 tensor"
     sections = tuple(sections)
-    if torch.compiler.is_compiling():                          # a node of the graph for each tensor
-        kid, sizes, _, _ = _rope_axes_plan(shapes[:n], shapes[n:-2], dtypes, devices, freqs.shape, positions.shape, sections, bool(half), order, backward)
-        for t, o, (num_bytes, value) in zip(tensors, outs, sizes):
-            if num_bytes:
-                _elementwise(kid, o, None, None, None, t, freqs, None, None, positions, value, 0, 0)
-        return outs
     key = ("rope_axes", n, tuple(shapes), tuple(dtypes), tuple(devices), sections, bool(half), order, backward)
     plan = _plans.get(key)
     if plan is None:
@@ -386,7 +388,6 @@ def _rope_axes_many(tensors, freqs, positions, sections, half: bool, order: str,
                            for (out, inp, size), (_, value) in zip(arrays, sizes)])
         device, stream = wrapper._device_and_stream(freqs)
         wrapper.library().sideaware_elementwise_batch(kid, n, packed, device, stream)
-    return outs
 
 
 def rope_axes_forward_many(tensors, freqs, positions, sections, half: bool = False, order: str = "blocks", outs=None):
@@ -428,6 +429,14 @@ def dropout_threshold(p: float) -> int:
 
 
 def _dropout(x: torch.Tensor, p: float, seed: torch.Tensor, residual: Optional[torch.Tensor], out: Optional[torch.Tensor]):
+    if torch.compiler.is_compiling():
+        out = _like(out, x, "out")
+        torch.ops.sideaware.dropout(x, p, seed, residual, out)
+        return out
+    return _dropout_launch(x, p, seed, residual, out)
+
+
+def _dropout_launch(x: torch.Tensor, p: float, seed: torch.Tensor, residual: Optional[torch.Tensor], out: Optional[torch.Tensor]):
     threshold = dropout_threshold(p)
     dtype = _ROPE_DTYPES.get(x.dtype)
     if dtype is None:
@@ -439,19 +448,29 @@ def _dropout(x: torch.Tensor, p: float, seed: torch.Tensor, residual: Optional[t
         assert residual.shape == x.shape and residual.dtype == x.dtype and residual.get_device() == device, "the residual is like the activation"
     out = _like(out, x, "out")
     if x.numel():
-        if torch.compiler.is_compiling():
-            _elementwise(_kernel("dropout", (dtype, residual is not None)), out, None, None, None, x, residual, None, None, seed, threshold, 0, 0)
-        else:
-            assert x.is_cuda, "x must be on the GPU"
-            kid = _kernel("dropout", (dtype, residual is not None))
-            size, to, first = x.numel() * x.element_size(), _aligned(out, "out"), _aligned(x, "x")
-            second = 0 if residual is None else _aligned(residual, "residual")
-            state = seed.data_ptr()
-            if 0 < abs(to - first) < size or second and 0 < abs(to - second) < size or to < state + 16 and state < to + size:
-                raise ValueError(_OVERLAP)
-            device, stream = wrapper._device_and_stream(x)
-            wrapper.library().sideaware_elementwise(kid, size, to, 0, 0, 0, first, second, 0, 0, state, threshold, 0, 0, device, stream)
+        assert x.is_cuda, "x must be on the GPU"
+        kid = _kernel("dropout", (dtype, residual is not None))
+        size, to, first = x.numel() * x.element_size(), _aligned(out, "out"), _aligned(x, "x")
+        second = 0 if residual is None else _aligned(residual, "residual")
+        state = seed.data_ptr()
+        if 0 < abs(to - first) < size or second and 0 < abs(to - second) < size or to < state + 16 and state < to + size:
+            raise ValueError(_OVERLAP)
+        device, stream = wrapper._device_and_stream(x)
+        wrapper.library().sideaware_elementwise(kid, size, to, 0, 0, 0, first, second, 0, 0, state, threshold, 0, 0, device, stream)
     return out
+
+
+def _dropout_node(x, p, seed, residual, out) -> None:
+    _dropout_launch(x, p, seed, residual, out)
+
+
+# Under torch.compile a call of these ops is one node of the graph, whose implementation is the eager call with all its
+# checks (by then tensors have addresses): the same launch, and the same refusals.
+_library = torch.library.Library("sideaware", "FRAGMENT")
+_library.define("rope_axes(Tensor[] tensors, Tensor freqs, Tensor positions, int[] sections, bool half, str order, bool backward, Tensor(a!)[] outs) -> ()")
+_library.define("dropout(Tensor x, float p, Tensor seed, Tensor? residual, Tensor(a!) out) -> ()")
+_library.impl("rope_axes", _rope_axes_launch, "CUDA")
+_library.impl("dropout", _dropout_node, "CUDA")
 
 
 def dropout_forward(x, p: float, seed, residual=None, out=None):
