@@ -445,6 +445,7 @@ struct CompiledKernel {
 struct KernelEntry {
     std::string header;         // fixed at registration
     int default_groups = 0;     // fixed at registration; 0: decide from occupancy
+    bool may_be_ragged = false; // fixed at registration: the text names RAGGED_TAIL (that it defines it, compiling says)
     // Serialises the compiles of this op: a first-use compile of one op (hundreds of
     // milliseconds) does not hold up launches of the others.
     std::mutex mu;
@@ -480,6 +481,7 @@ static int publish_entry_locked(const std::string& header, int default_groups) {
     e->header = header;
     e->function_name = kernel_name_of(header);
     e->default_groups = default_groups > 0 ? default_groups : 0;
+    e->may_be_ragged = header.find("RAGGED_TAIL") != std::string::npos;
     g_entries[id].store(e, std::memory_order_release);
     g_entry_count.store(id + 1, std::memory_order_release);
     return id;
@@ -531,6 +533,13 @@ static KernelEntry* find_entry(int kernel_id) {
         return nullptr;
     }
     return g_entries[kernel_id].load(std::memory_order_acquire);
+}
+
+// Whether arrays of this op may end inside a vector, as far as is known before it is compiled.
+static bool may_be_ragged(int kernel_id) {
+    ensure_builtin();
+    return kernel_id >= 0 && kernel_id < g_entry_count.load(std::memory_order_acquire) &&
+           g_entries[kernel_id].load(std::memory_order_acquire)->may_be_ragged;
 }
 
 // Builds the instantiation (sideaware.cu:772-813) and publishes it, successful or not: a failed
@@ -974,9 +983,9 @@ void sideaware_elementwise(int kernel_id, size_t num_bytes,
     if (num_bytes == 0 || (out0 == nullptr && in0 == nullptr)) return;
     DeviceContext* ctx = get_context(device);
     if (!ctx) return;
-    // an op that defines RAGGED_TAIL takes any whole number of elements; which ops do is known once
-    // they are compiled
-    if (!check_vector_alignment("elementwise", out0, in0, num_bytes % 16 && kernel_id != 0 ? 0 : num_bytes)) return;
+    // an op that defines RAGGED_TAIL takes any whole number of elements; others are refused here, before anything is
+    // compiled or captured for them
+    if (!check_vector_alignment("elementwise", out0, in0, num_bytes % 16 && may_be_ragged(kernel_id) ? 0 : num_bytes)) return;
 
     const Tuning t = tuning_snapshot();
     const int variant = variant_for(num_bytes, num_bytes, out0, in0, split_lines(out0, out1, out2, out3), t);
