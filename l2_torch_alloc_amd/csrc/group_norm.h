@@ -156,7 +156,9 @@ inline GroupNormPlan plan_group_norm(long long batch, long long pixels, int chan
     } else {
         cut(most_units);
         const long long step = p.rows;
-        // as many workgroups as the device holds at once, and no second, half-empty turn; at least four pixels a lane
+        // no more workgroups than the device holds at once, unless the (sample, slab) pairs are more already, and at least
+        // four pixels a lane.  From half as many pairs on each has one chunk, so places stay empty, and behind a full turn a
+        // nearly empty one may run: forward, 257 samples of 4096 pixels of 320 channels 449 us, 256 samples 391; 513 821, 512 765
         const long long want = 2ll * num_cus / (batch * p.slabs), most = gn_ceil(pixels, 4 * step);
         const long long least = gn_ceil(pixels, step * kGroupNormMaxLanePixels);
         long long k = want < most ? want : most;

@@ -17,7 +17,7 @@
 // A lane keeps one vector of channels and walks pixels, so all accesses of a wave are runs of whole
 // vectors and its sums are per channel, in registers; whatever the number of channels in a group is,
 // groups are only told apart when the sums are added up.  The sums of squares are of differences to
-// the lane's first value of the channel, so that a mean far from zero costs no digits, and become
+// the lane's first value of the channel's group, so that a mean far from zero costs no digits, and become
 // doubles before lanes are added: every sum of doubles below is in a fixed order, so results do not
 // depend on which workgroup came first.
 #include <hip/hip_runtime.h>

@@ -394,7 +394,7 @@ def rope_axes_forward_many(tensors, freqs, positions, sections, half: bool = Fal
     """RoPE with a position of 1 to 3 axes (the time, height and width of an image's or video's patch) of
     several (B, T, heads, head_dim) tensors in ONE launch: q and k of a grouped-query model (different
     head counts, same B, T, head_dim and dtype).  In place unless ``outs`` is given; returns the outputs.  An
-    output is its own tensor or shares no memory with any other.
+    output is its own tensor or shares no memory with any other, the table and the positions among them.
 
     ``freqs``: the (rows, head_dim) fp32 table of the ops with one position (``freqs_cis_table``, or
     ``freqs_cis_axes_table`` for axes with frequencies of their own), with a row for every position that
@@ -479,7 +479,7 @@ def dropout_forward(x, p: float, seed, residual=None, out=None):
     is computed from the element's index and ``seed``, an int64 device tensor (seed, offset), and never
     stored: pass the same two to :func:`dropout_backward`.  A launch captured into a graph reads the
     tensor at every replay, so advancing the offset in place gives each replay a new mask.
-    ``x`` may have any number of elements.  ``out`` may be ``x`` or ``residual``, but not overlap them otherwise."""
+    ``x`` may have any number of elements.  ``out`` may be ``x`` or ``residual``, but not overlap them otherwise, nor ``seed``."""
     return _dropout(x, p, seed, residual, out)
 
 
